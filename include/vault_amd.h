@@ -294,6 +294,90 @@ int64_t vgx_attn_prefill_workspace_bytes(int64_t H, int64_t G);
 int vgx_attn_prefill_ws(int kv_dtype, int q_dtype, int out_dtype, const vgx_attn_block *blocks, int n_blocks, int64_t H,
                         int64_t G, int64_t D, float scale, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------- paged 8-bit K/V cache -------- */
+
+/* A cache of keys and values in 8 bits, in pages of `page` tokens that a page table hands out to sequences of any
+ * length.  One fp32 scale per (layer, page, kv head) for K and one for V; a value is code * scale with
+ *   VGX_I8:   code = byte - 128, in [-127, 127]
+ *   VGX_E4M3: code = the float8 e4m3 (fn) value of the byte, |code| <= 448.
+ * K: [n_layers][n_pages][G][page][D] bytes; V with tokens contiguous: [n_layers][n_pages][G][D][page]; scales
+ * [n_layers][n_pages][G], not negative.  Layers lie `layer_stride` bytes (a multiple of 16; scales:
+ * `scale_layer_stride` floats) apart, all else is contiguous.  D in {64, 128}; page in {16, 32, 64, 128, 256}; k and v
+ * 16-byte aligned.
+ *
+ * Page tables are device int32 [sequences][table_cols] (row stride ldt): entry j of a sequence's row is the page of its
+ * tokens [j * page, (j + 1) * page).  An entry outside [0, n_pages), or past table_cols, is no page: nothing is written
+ * there and its tokens are not visible, so entries of pages that a sliding window has left behind may be -1.  Pages may
+ * be shared by sequences as long as only one of them writes to a page in a call.
+ * No counterpart in the reference, whose state tensors are dense and whose batches are in lockstep. */
+enum { VGX_I8 = 16, VGX_E4M3 = 17 };
+
+typedef struct vgx_paged_kv {
+    int fmt;                    /* VGX_I8 or VGX_E4M3 */
+    uint8_t *k;
+    uint8_t *v;
+    float *k_scale;
+    float *v_scale;
+    int64_t n_layers;
+    int64_t n_pages;
+    int64_t G;
+    int64_t page;
+    int64_t D;
+    int64_t layer_stride;
+    int64_t scale_layer_stride;
+} vgx_paged_kv;
+
+/* New tokens into the pages of one layer: N rows k / v of [G][D] elements (row strides ldk / ldv; dtype VGX_F32 or
+ * VGX_BF16 for k, v, q and q_out alike), rows [q_start[b], q_start[b + 1]) belonging to sequence b < B (device int32
+ * [B + 1], not decreasing; NULL: N == B, one row each), at the positions start[b] (device int32), start[b] + 1, ...
+ * Rows from q_start[B] on, and tokens at a position below 0 or without a page, are skipped.
+ * With `rope` (fp32 rows [cos(D/2) | sin(D/2)], row stride rope_ld; row p for position p) keys are rotated on the way
+ * (fp32 products and sums rounded once); a position outside [0, rope_rows) counts as NaN.
+ * A page's scale becomes max(its scale, if it holds tokens before start[b]; amax / 127 or amax / 448 over its new
+ * tokens), amax the largest magnitude of head g; new codes are round(fp32(x / scale)), to nearest even, and the codes of
+ * the older tokens are rounded again when the scale grew.  A non-finite value makes the scale of its page and head NaN.
+ * q (may be NULL; [H][D] per row, row stride ldq) is rotated into q_out (row stride ldqo; may be q itself).  Rows must
+ * be 16-byte aligned. */
+int vgx_paged_append(const vgx_paged_kv *kv, int64_t layer, int dtype, const void *k, int64_t ldk, const void *v,
+                     int64_t ldv, int64_t N, const int32_t *table, int64_t ldt, int64_t table_cols, const int32_t *start,
+                     const int32_t *q_start, int64_t B, const float *rope, int64_t rope_ld, int64_t rope_rows,
+                     const void *q, int64_t ldq, void *q_out, int64_t ldqo, int64_t H, void *stream);
+
+/* Attention of N query rows over the pages of one layer: rows as in vgx_paged_append; sequence b holds lens[b] tokens
+ * (device int32), its n_b queries being its last n_b positions, query t at position p = lens[b] - n_b + t.
+ *   out[row, h] = softmax_j(scale * q[row, h] . k_j) v_j    over keys j <= p of head h / (H / G) with a page and, when
+ * window > 0, with j > p - window or j < n_sink (the first tokens that stay visible).  A row that sees no key gets
+ * zeros; rows from q_start[B] on are left as they are.  q and out: dtype VGX_F32 (fp32-level results) or VGX_BF16 (fp32
+ * sums, probabilities in fp16); head h of a row at h * D.  Rows must be 16-byte aligned, H a multiple of G.
+ * max_new: the most rows of a sequence, max_keys: the most keys of one (hints that choose how the work is split;
+ * results do not depend on their truth beyond rounding).  workspace: vgx_paged_attn_workspace_bytes of the same
+ * arguments, 16-byte aligned, any content; calls sharing one must not overlap in time.  N, B, max_keys <= 2^30 and
+ * table_cols * page < 2^30. */
+int64_t vgx_paged_attn_workspace_bytes(int64_t N, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_new,
+                                       int64_t max_keys, int64_t window, int64_t n_sink);
+int vgx_paged_attn(const vgx_paged_kv *kv, int64_t layer, int dtype, const void *q, int64_t ldq, void *out, int64_t ldo,
+                   int64_t N, int64_t H, const int32_t *table, int64_t ldt, int64_t table_cols, const int32_t *lens,
+                   const int32_t *q_start, int64_t B, int64_t max_new, int64_t max_keys, int64_t window, int64_t n_sink,
+                   float scale, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Dequantized rows of every layer: k_out / v_out [n_layers][B][G][n][D] (dtype VGX_F32 or VGX_BF16; 16-byte aligned)
+ * receive positions [first[b], first[b] + n) of sequence b (first, lens: device int32); zeros at positions below 0, at
+ * or past lens[b], or without a page.  Brings a sequence back to the dense runs of vgx_attn_decode / vgx_attn_prefill. */
+int vgx_paged_read(const vgx_paged_kv *kv, int dtype, const int32_t *table, int64_t ldt, int64_t table_cols,
+                   const int32_t *first, const int32_t *lens, int64_t B, int64_t n, void *k_out, void *v_out,
+                   void *stream);
+
+/* Beam search's reordering: sequences in groups of K beams (K <= 64; row b * K + i is beam i of group b), new beam i of a
+ * group continuing beam parents[b * K + i] (a value outside [0, K) counts as i).  lens_out = the parents' lengths;
+ * table_out rows: the parent's entries below lens / page, then the page that the next token goes to, then the row's own
+ * entries past its own such page (-1 between).  Every beam owns the page at entry lens / page of its row before the
+ * call, and does after it: the first beam that continues a parent takes that page over, every further one gets the page
+ * of a beam that nothing continues (both in ascending order), into which all layers of the parent's page and its scales
+ * are copied.  Earlier pages become shared.  table_out must not overlap table, nor lens_out lens. */
+int vgx_paged_reorder(const vgx_paged_kv *kv, const int32_t *table, int64_t ldt, int64_t table_cols, const int32_t *lens,
+                      const int32_t *parents, int64_t groups, int64_t K, int32_t *table_out, int64_t ldt_out,
+                      int32_t *lens_out, void *stream);
+
 /* ---------------------------------------------------------------- small fused ops -------------- */
 
 /* RMSNorm rows: y[r, :] = w * (x[r, :] / sqrt(mean(x[r, :]^2) + eps)).
@@ -498,6 +582,20 @@ int vgx_argmax(const float *logits, int64_t ld, int64_t B, int64_t V, int64_t *o
 int64_t vgx_sample_topk_workspace_bytes(int64_t B, int64_t V);
 int vgx_sample_topk(const float *logits, int64_t ld, int64_t B, int64_t V, int64_t k, float temp, uint64_t *rng,
                     int64_t *out, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Beam search's choice: for groups of K beams (K <= 64; logits row b * K + k, row stride ld) the K best of the K * V
+ * continuations by total(k, v) = scores[b * K + k] + x_v - log(sum_u exp(x_u)), in descending order, ties to the smaller
+ * k * V + v.  A beam with done[b * K + k] != 0 (done may be NULL) has the one continuation (k, eos) with total =
+ * its score.  Totals that are NaN or -inf are no candidates.  Writes scores_out (fp32), parents (the beam k), tokens
+ * (int64) and, unless NULL, done_out (the parent's flag, or token == eos); where candidates run out: -inf, the beam's
+ * own index, token -1, done 1.  eos < 0: none (done must then be NULL).  V <= 2^19.  scores_out and done_out may be
+ * scores and done.  workspace: vgx_beam_select_workspace_bytes, 16-byte aligned, any content; calls sharing one must
+ * not overlap in time.  Beside vgx_argmax and vgx_sample_topk; no counterpart in the reference, which samples one
+ * sequence (runtime/vault3.c:3198-3230). */
+int64_t vgx_beam_select_workspace_bytes(int64_t groups, int64_t K, int64_t V);
+int vgx_beam_select(const float *logits, int64_t ld, int64_t groups, int64_t K, int64_t V, const float *scores,
+                    const uint8_t *done, int64_t eos, float *scores_out, int32_t *parents, int64_t *tokens,
+                    uint8_t *done_out, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------- segment-memory scorer -------- */
 

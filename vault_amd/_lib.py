@@ -19,6 +19,7 @@ ERRORS = {
 }
 
 F32, F16, BF16, Q8_0, Q4_0 = 0, 1, 2, 8, 9
+I8, E4M3 = 16, 17          # code formats of the paged K/V cache
 EPI_STORE, EPI_ACCUM, EPI_SWIGLU = 0, 1, 2
 STEP_SLOT, STEP_TABLE_ROW, STEP_SINK_SLOT, STEP_N_CUR, STEP_WORDS = 0, 1, 2, 3, 4
 SEG_MEM_CNT, SEG_ID_OFFSET, SEG_CUR_ID, SEG_LEN, SEG_WORDS = 0, 1, 2, 3, 4
@@ -92,6 +93,15 @@ _SIGS = {
     "vgx_attn_prefill_planes_bytes": (I64, [I32, P, I32, I64, I64]),
     "vgx_attn_prefill_planes": (I32, [I32, I32, I32, P, I32, I64, I64, I64, F, P, I64, P]),
     "vgx_attn_prefill_ws": (I32, [I32, I32, I32, P, I32, I64, I64, I64, F, P, I64, P]),
+    "vgx_paged_append": (I32, [P, I64, I32, P, I64, P, I64, I64, P, I64, I64, P, P, I64, P, I64, I64, P, I64, P, I64, I64,
+                               P]),
+    "vgx_paged_attn_workspace_bytes": (I64, [I64, I64, I64, I64, I64, I64, I64, I64, I64]),
+    "vgx_paged_attn": (I32, [P, I64, I32, P, I64, P, I64, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, F, P, I64,
+                             P]),
+    "vgx_paged_read": (I32, [P, I32, P, I64, I64, P, P, I64, I64, P, P, P]),
+    "vgx_paged_reorder": (I32, [P, P, I64, I64, P, P, I64, I64, P, I64, P, P]),
+    "vgx_beam_select_workspace_bytes": (I64, [I64, I64, I64]),
+    "vgx_beam_select": (I32, [P, I64, I64, I64, I64, P, P, I64, P, P, P, P, P, I64, P]),
     "vgx_rmsnorm": (I32, [P, I64, P, P, I64, I64, I64, F, P]),
     "vgx_rope_qkv_write": (I32, [I32, P, I64, P, I64, P, I64, I64, I64, I64, I64, P, I64, P, P, P, I64, I64, P, P, I64,
                                  I64, I64, P]),
@@ -129,6 +139,13 @@ class AttnBlock(C.Structure):
                 ("ldo", C.c_int64), ("o_hstride", C.c_int64), ("n_q", C.c_int64), ("causal_base", C.c_int64),
                 ("n_runs", C.c_int), ("runs", KVRun * 4), ("bias", C.c_void_p), ("bias_head_row", C.c_void_p),
                 ("bias_ldq", C.c_int64), ("bias_rstride", C.c_int64), ("bias_run", C.c_int)]
+
+
+class PagedKV(C.Structure):
+    """vgx_paged_kv (include/vault_amd.h)."""
+    _fields_ = [("fmt", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("n_layers", C.c_int64), ("n_pages", C.c_int64), ("G", C.c_int64),
+                ("page", C.c_int64), ("D", C.c_int64), ("layer_stride", C.c_int64), ("scale_layer_stride", C.c_int64)]
 
 
 class ScoreSide(C.Structure):

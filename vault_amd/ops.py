@@ -5,6 +5,7 @@ into the HIP library (no torch fallback).  Tensors must live on a ROCm device.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import sys
 from typing import Optional, Tuple
@@ -28,6 +29,14 @@ def payload_bytes(dtype: int, rows: int, cols: int) -> int:
 
 def _stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """A context in which ``dev`` is the current device (a launch goes to the current one, whatever its stream)."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -774,3 +783,41 @@ def sample_topk(logits: torch.Tensor, k: int, temp: float, rng: torch.Tensor,
     L.check(lib.vgx_sample_topk(logits.data_ptr(), logits.stride(0), B, V, int(k), float(temp), rng.data_ptr(),
                                 out.data_ptr(), buf.data_ptr(), buf.numel(), _stream(logits.device)), "vgx_sample_topk")
     return out
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: Optional[torch.Tensor] = None, eos: int = -1,
+                ws: Optional["Workspace"] = None):
+    """Beam search's choice (vgx_beam_select): for B groups of K beams, the K best continuations by
+    score + log-softmax(logits), ties to the smaller beam * V + token.  logits [B * K, V] fp32, scores [B, K] fp32 (-inf:
+    no candidates), done uint8 [B, K] or None: finished beams, which continue as (beam, eos) at their score.  Returns
+    (scores fp32, parents int32, tokens int64, done uint8), each [B, K], on the device; where candidates run out score
+    -inf, the beam itself, token -1, done 1.  With ``ws`` (a Workspace, one per stream) no scratch is allocated."""
+    _need(logits, torch.float32, "logits")
+    _need(scores, torch.float32, "scores")
+    if logits.dim() != 2 or scores.dim() != 2 or logits.shape[0] != scores.numel():
+        raise ValueError("logits must be [B * K, V] and scores [B, K]")
+    if logits.stride(1) != 1 or not scores.is_contiguous():
+        raise ValueError("logits rows and scores must be contiguous")
+    dev = logits.device
+    if scores.device != dev:
+        raise ValueError("logits and scores must be on one device")
+    if done is not None:
+        _need(done, torch.uint8, "done")
+        if done.shape != scores.shape or not done.is_contiguous() or done.device != dev:
+            raise ValueError("done must be a contiguous uint8 tensor like scores")
+        if eos < 0:
+            raise ValueError("finished beams need eos")
+    (B, K), V = scores.shape, logits.shape[1]
+    lib = L.load()
+    need = int(lib.vgx_beam_select_workspace_bytes(B, K, V))
+    L.check(min(need, 0), "vgx_beam_select_workspace_bytes")
+    buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=dev)
+    out = torch.empty_like(scores)
+    parents = torch.empty(B, K, dtype=torch.int32, device=dev)
+    tokens = torch.empty(B, K, dtype=torch.int64, device=dev)
+    done_out = torch.empty(B, K, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        L.check(lib.vgx_beam_select(logits.data_ptr(), logits.stride(0), B, K, V, scores.data_ptr(), _ptr(done), eos,
+                                    out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), done_out.data_ptr(),
+                                    buf.data_ptr(), buf.numel(), _stream(dev)), "vgx_beam_select")
+    return out, parents, tokens, done_out

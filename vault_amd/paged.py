@@ -1,0 +1,280 @@
+"""A paged K/V cache in 8 bits for batches of sequences of different lengths, and the operators on it.
+
+``PagedKV`` holds the pages of all layers; page tables (device int32 [sequences, entries]) hand them out.  A decode step
+is ``append`` (rotate the new keys and queries, round K / V to 8 bits into their pages) and ``attend`` per layer; both also
+take many new tokens per sequence (prompts, chunks, drafted tokens).  ``read`` brings rows back to the dense tensors of
+``ops.attn_decode`` / ``ops.attn_prefill``; ``reorder`` follows a beam search's choice (``ops.beam_select``).
+
+Batches of new tokens are packed: ``q_start`` (device int32 [B + 1]) names the rows [q_start[b], q_start[b + 1]) of
+sequence b; None: one row per sequence.  Everything is ordered on the current stream of the tensors' device and can be
+captured into a graph (outputs then are the caller's, or live in the graph's pool).  Lengths, positions and tables are
+read on the device, so a captured step follows what they hold at replay.  Device values that make no sense (a page id
+outside the cache, lengths past the table) are not errors: see include/vault_amd.h for what each operator does with them.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib as L
+from .ops import KV_DTYPES, Workspace, _on, _ptr, _stream
+
+I8, E4M3 = L.I8, L.E4M3
+PAGES = (16, 32, 64, 128, 256)
+
+
+class PagedKV:
+    """Pages of 8-bit K / V codes with one scale per (layer, page, kv head).
+
+    k: uint8 [layers, pages, G, page, D]; v: uint8 [layers, pages, G, D, page] (tokens contiguous); k_scale / v_scale:
+    fp32 [layers, pages, G], not negative.  ``fmt``: I8 (value = (byte - 128) * scale) or E4M3 (float8_e4m3fn * scale).
+    D 64 or 128, page 16 .. 256 (a power of two).  Layers may lie apart; all else must be contiguous."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, fmt: int):
+        if fmt not in (I8, E4M3):
+            raise ValueError("fmt must be I8 or E4M3")
+        if k.dim() != 5:
+            raise ValueError("k must be [layers, pages, G, page, D]")
+        n, pages, G, P, D = k.shape
+        if min(k.shape) < 1 or D not in (64, 128) or P not in PAGES:
+            raise ValueError(f"head dim 64 or 128 and pages of {PAGES} tokens, got {D} and {P}")
+        if v.shape != (n, pages, G, D, P):
+            raise ValueError("v must be [layers, pages, G, D, page]")
+        if k_scale.shape != (n, pages, G) or v_scale.shape != k_scale.shape:
+            raise ValueError("scales must be [layers, pages, G]")
+        for t, dt, name in ((k, torch.uint8, "k"), (v, torch.uint8, "v"), (k_scale, torch.float32, "k_scale"),
+                            (v_scale, torch.float32, "v_scale")):
+            if not t.is_cuda:
+                raise ValueError(f"{name} must be a device tensor")
+            if t.dtype != dt:
+                raise ValueError(f"{name} must be {dt}, got {t.dtype}")
+            if t.device != k.device:
+                raise ValueError("the cache must be on one device")
+            if not t[0].is_contiguous():
+                raise ValueError(f"{name}: a layer must be contiguous")
+        if n > 1 and (v.stride(0) != k.stride(0) or v_scale.stride(0) != k_scale.stride(0)):
+            raise ValueError("k and v, and their scales, need equal layer strides")
+        self.k, self.v, self.k_scale, self.v_scale, self.fmt = k, v, k_scale, v_scale, fmt
+        self.n_layers, self.n_pages, self.G, self.page, self.D = n, pages, G, P, D
+        self.device = k.device
+        self._c = L.PagedKV(fmt, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, pages, G, P, D,
+                            k.stride(0) if n > 1 else pages * G * P * D, k_scale.stride(0) if n > 1 else pages * G)
+        self._ref = C.addressof(self._c)
+
+    @classmethod
+    def empty(cls, n_layers: int, n_pages: int, G: int, D: int, device, page: int = 64, fmt: int = I8) -> "PagedKV":
+        """Pages of zeros."""
+        shape = (n_layers, n_pages, G)
+        zero = 128 if fmt == I8 else 0
+        full = lambda *tail: torch.full((*shape, *tail), zero, dtype=torch.uint8, device=device)  # noqa: E731
+        return cls(full(page, D), full(D, page), torch.zeros(shape, device=device), torch.zeros(shape, device=device),
+                   fmt)
+
+
+def _words(t: torch.Tensor, shape, dev, name: str) -> None:
+    if t.dtype != torch.int32 or t.device != dev:
+        raise ValueError(f"{name} must be an int32 tensor on the cache's device")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _table(t: torch.Tensor, dev, name: str = "table") -> None:
+    if t.dtype != torch.int32 or t.device != dev or t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError(f"{name} must be int32 [sequences, entries] on the cache's device")
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"{name} rows must be contiguous and apart")
+
+
+def _rows(t: torch.Tensor, heads: Optional[int], D: int, dtype, dev, name: str) -> torch.Tensor:
+    """[N, heads, D] with contiguous heads and 16-byte aligned rows (a copy where the view is not)."""
+    if t.dim() != 3 or t.shape[2] != D or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [N, {heads if heads is not None else 'H'}, {D}], got {tuple(t.shape)}")
+    if t.dtype != dtype or t.device != dev:
+        raise ValueError(f"{name} must be {dtype} on the cache's device")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D) or t.data_ptr() % 16 or \
+            (t.shape[0] > 1 and (t.stride(0) * t.element_size() % 16 or t.stride(0) < t.shape[1] * D)):
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t
+
+
+def _dest(t: torch.Tensor, like: torch.Tensor, name: str) -> None:
+    """An output that rows are written into, in place."""
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on the cache's device")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]) or t.data_ptr() % 16 or \
+            (t.shape[0] > 1 and (t.stride(0) * t.element_size() % 16 or t.stride(0) < t.shape[1] * t.shape[2])):
+        raise ValueError(f"{name} needs contiguous heads and 16-byte aligned rows")
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _batch(table: torch.Tensor, q_start: Optional[torch.Tensor], N: int, dev) -> int:
+    B = table.shape[0]
+    if q_start is None:
+        if N != B:
+            raise ValueError(f"without q_start every sequence has one row: {N} rows for {B} sequences")
+    else:
+        _words(q_start, (B + 1,), dev, "q_start")
+    return B
+
+
+def _layer(kv: PagedKV, layer: int) -> None:
+    if not 0 <= layer < kv.n_layers:
+        raise ValueError(f"layer {layer} of {kv.n_layers}")
+
+
+def append(kv: PagedKV, layer: int, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, *,
+           rope: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+           q_start: Optional[torch.Tensor] = None, max_new: Optional[int] = None) -> Optional[torch.Tensor]:
+    """New tokens into the pages of ``layer`` (vgx_paged_append).
+
+    k, v [N, G, D] fp32 or bf16; sequence b's rows take the positions start[b], start[b] + 1, ... (start int32 [B]: the
+    tokens that it holds already).  ``rope`` fp32 [positions, D], rows [cos | sin]: keys are rotated by their position's
+    row.  With q [N, H, D] (dtype of k) the queries are rotated too, into ``q_out`` (may be q; a new tensor by default),
+    which is returned.  A sequence's pages must be in its table row; a page that is written must be in one row only.
+    ``max_new`` is not needed and only accepted for symmetry with ``attend``."""
+    dev, G, D = kv.device, kv.G, kv.D
+    _layer(kv, layer)
+    _table(table, dev)
+    if k.dtype not in KV_DTYPES:
+        raise ValueError("k must be fp32 or bf16")
+    k, v = _rows(k, G, D, k.dtype, dev, "k"), _rows(v, G, D, k.dtype, dev, "v")
+    N = k.shape[0]
+    if v.shape[0] != N:
+        raise ValueError("k and v must have the same rows")
+    B = _batch(table, q_start, N, dev)
+    _words(start, (B,), dev, "start")
+    rope_ld = rope_rows = H = 0
+    if rope is not None:
+        if rope.dtype != torch.float32 or rope.device != dev or rope.dim() != 2 or rope.shape[1] != D:
+            raise ValueError("rope must be fp32 [positions, D] on the cache's device")
+        if rope.stride(1) != 1 or rope.stride(0) % 4 or rope.data_ptr() % 16:
+            raise ValueError("rope rows must be contiguous and 16-byte aligned")
+        rope_ld, rope_rows = rope.stride(0), rope.shape[0]
+    src = None
+    if q is not None:
+        src = _rows(q, None, D, k.dtype, dev, "q")
+        if src.shape[0] != N or src.shape[1] < 1:
+            raise ValueError("q must have the rows of k")
+        H = src.shape[1]
+        if q_out is None:
+            q_out = torch.empty(N, H, D, dtype=k.dtype, device=dev)
+        else:
+            _dest(q_out, q, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    with _on(dev):
+        L.check(L.load().vgx_paged_append(
+            kv._ref, layer, KV_DTYPES[k.dtype], k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), N, table.data_ptr(),
+            table.stride(0) if B > 1 else table.shape[1], table.shape[1], start.data_ptr(), _ptr(q_start), B, _ptr(rope),
+            rope_ld, rope_rows, _ptr(src), _ld(src) if src is not None else 0, _ptr(q_out),
+            _ld(q_out) if q_out is not None else 0, H, _stream(dev)), "vgx_paged_append")
+    return q_out
+
+
+def attend(kv: PagedKV, layer: int, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *,
+           q_start: Optional[torch.Tensor] = None, max_new: Optional[int] = None, max_keys: Optional[int] = None,
+           window: int = 0, n_sink: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+           ws: Optional[Workspace] = None) -> torch.Tensor:
+    """Attention over the pages of ``layer`` (vgx_paged_attn).
+
+    q [N, H, D] fp32 or bf16, rotated; lens int32 [B]: tokens that sequence b holds, its queries being its last ones (so
+    after an append, lens = start + new tokens).  Every query sees the keys up to its own position, with ``window`` > 0
+    only the last ``window`` of them and the first ``n_sink`` tokens.  Returns [N, H, D] in q's dtype; a query that sees
+    nothing gets zeros, rows behind the last sequence stay as they were.  ``max_new`` / ``max_keys``: the most rows and
+    keys of one sequence, hints for the split of the work (by default what the shapes allow).  ``ws``: a Workspace of this
+    stream; without it scratch is allocated."""
+    dev, G, D = kv.device, kv.G, kv.D
+    _layer(kv, layer)
+    _table(table, dev)
+    if q.dtype not in KV_DTYPES:
+        raise ValueError("q must be fp32 or bf16")
+    src = _rows(q, None, D, q.dtype, dev, "q")
+    N, H = src.shape[0], src.shape[1]
+    if H < 1 or H % G:
+        raise ValueError(f"{H} query heads for {G} kv heads")
+    B = _batch(table, q_start, N, dev)
+    _words(lens, (B,), dev, "lens")
+    if window < 0 or n_sink < 0:
+        raise ValueError("window and n_sink must not be negative")
+    if out is None:
+        out = torch.empty(N, H, D, dtype=q.dtype, device=dev)
+    else:
+        _dest(out, q, "out")
+    most = 1 if q_start is None else N if max_new is None else max_new
+    keys = table.shape[1] * kv.page
+    keys = keys if max_keys is None else min(max_keys, keys)
+    if most < 0 or keys < 0:
+        raise ValueError("max_new and max_keys must not be negative")
+    lib = L.load()
+    need = int(lib.vgx_paged_attn_workspace_bytes(N, B, H, G, D, most, keys, window, n_sink))
+    L.check(min(need, 0), "vgx_paged_attn_workspace_bytes")
+    buf = None
+    if need > 0:
+        buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=dev)
+        if buf.device != dev:
+            raise ValueError("the workspace must be on the cache's device")
+    with _on(dev):
+        L.check(lib.vgx_paged_attn(
+            kv._ref, layer, KV_DTYPES[q.dtype], src.data_ptr(), _ld(src), out.data_ptr(), _ld(out), N, H,
+            table.data_ptr(), table.stride(0) if B > 1 else table.shape[1], table.shape[1], lens.data_ptr(),
+            _ptr(q_start), B, most, keys, window, n_sink, float(scale if scale is not None else D ** -0.5), _ptr(buf),
+            buf.numel() if buf is not None else 0, _stream(dev)), "vgx_paged_attn")
+    return out
+
+
+def read(kv: PagedKV, table: torch.Tensor, first: torch.Tensor, n: int, lens: torch.Tensor,
+         dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Dequantized rows of all layers (vgx_paged_read): (k, v), each [layers, B, G, n, D] fp32 or bf16, row i of sequence
+    b being position first[b] + i; zeros at positions below 0 or at or past lens[b], and where the table has no page.
+    Keys come back rotated as they were stored."""
+    dev = kv.device
+    _table(table, dev)
+    B = table.shape[0]
+    _words(first, (B,), dev, "first")
+    _words(lens, (B,), dev, "lens")
+    if dtype not in KV_DTYPES:
+        raise ValueError("dtype must be fp32 or bf16")
+    if n < 0:
+        raise ValueError("n must not be negative")
+    k = torch.empty(kv.n_layers, B, kv.G, n, kv.D, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    with _on(dev):
+        L.check(L.load().vgx_paged_read(
+            kv._ref, KV_DTYPES[dtype], table.data_ptr(), table.stride(0) if B > 1 else table.shape[1], table.shape[1],
+            first.data_ptr(), lens.data_ptr(), B, n, k.data_ptr(), v.data_ptr(), _stream(dev)), "vgx_paged_read")
+    return k, v
+
+
+def reorder(kv: PagedKV, table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, table_out: torch.Tensor,
+            lens_out: torch.Tensor) -> None:
+    """After a beam search's choice: beam i of group b continues beam parents[b, i] (vgx_paged_reorder).
+
+    table [B * K, entries] and lens [B * K] are the beams' before, table_out / lens_out (other tensors) after.  Full pages
+    become shared; the page that the next token goes to is owned by one beam before and after (give every beam its own
+    before the call): the first child takes its parent's over, further children get copies in the pages of beams that
+    nothing continues.  Entries past that page stay the row's own.  A page stays in use until no table names it."""
+    dev = kv.device
+    if parents.dim() != 2:
+        raise ValueError("parents must be int32 [groups, K]")
+    B, K = parents.shape
+    _words(parents, (B, K), dev, "parents")
+    _table(table, dev)
+    _table(table_out, dev, "table_out")
+    if table.shape[0] != B * K or table_out.shape != table.shape:
+        raise ValueError("table and table_out must have a row per beam")
+    _words(lens, (B * K,), dev, "lens")
+    _words(lens_out, (B * K,), dev, "lens_out")
+    if table_out.data_ptr() == table.data_ptr() or lens_out.data_ptr() == lens.data_ptr():
+        raise ValueError("table_out and lens_out must be other tensors than table and lens")
+    with _on(dev):
+        L.check(L.load().vgx_paged_reorder(
+            kv._ref, table.data_ptr(), table.stride(0) if B * K > 1 else table.shape[1], table.shape[1], lens.data_ptr(),
+            parents.data_ptr(), B, K, table_out.data_ptr(), table_out.stride(0) if B * K > 1 else table.shape[1],
+            lens_out.data_ptr(), _stream(dev)), "vgx_paged_reorder")
