@@ -11,6 +11,8 @@
 // arranged by lane) is compacted into shared memory and ranked there.
 #include "common.h"
 
+#include <algorithm>
+
 using namespace vgx;
 
 namespace {
@@ -196,20 +198,25 @@ struct JoinArgs {
     int V, K, chunks;
 };
 
-// One workgroup per group of beams.  Dynamic shared memory: `cells` (a power of two, at least K * chunks and K * K)
-// totals and as many tags.
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(const JoinArgs A, int cells) {
+// One workgroup per group of beams.  Dynamic shared memory: `cells` totals and as many tags, at least K * chunks and K * K.
+// COUNT: up to 1024 of both are ranked by counting what comes before them (152 heads of 8 beams over 19 chunks: 5.5 us for
+// the launch); more are sorted, cells being a power of two (the same: 26 us).
+template <int THREADS, bool COUNT>
+__global__ __launch_bounds__(THREADS) void join_kernel(const JoinArgs A, int cells) {
     extern __shared__ uint64_t tot[];
     uint32_t *tag = reinterpret_cast<uint32_t *>(tot + cells);
     __shared__ double lse[kMaxK];
     __shared__ float score[kMaxK];
-    __shared__ uint8_t fin[kMaxK];
+    __shared__ uint32_t fin[kMaxK];
     __shared__ int pick[kMaxK];
     const int tid = threadIdx.x, lane = tid & 63, K = A.K, C = A.chunks;
     const int64_t base = (int64_t)blockIdx.x * K;
-    for (int k = tid >> 6; k < K; k += kJoinThreads / 64) {
+    // this thread's head, requested before the sums are waited for
+    const uint64_t head = COUNT && tid < K * C ? A.lists[(base * C + tid) * K] : 0ull;
+    for (int k = tid >> 6; k < K; k += THREADS / 64) {
         const float2 *s = A.sums + (base + k) * C;
         const bool f = A.done != nullptr && A.done[base + k] != 0;
+        const float sc = A.scores[base + k];
         float m = -INFINITY;
         double sum = 0.0;
         if (!f) {
@@ -217,79 +224,111 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const JoinArgs A, in
             m = wave_max(m);
             for (int c = lane; c < C; c += 64) {
                 const float2 v = s[c];
-                sum += v.x == -INFINITY ? (double)v.y : (double)v.y * exp((double)v.x - (double)m);
+                sum += v.x == -INFINITY ? (double)v.y : (double)v.y * (double)__expf(v.x - m);
             }
 #pragma unroll
             for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, kWave);
         }
         if (lane == 0) {
             lse[k] = (double)m + log(sum);
-            score[k] = A.scores[base + k];
-            fin[k] = f ? 1 : 0;
+            score[k] = sc;
+            fin[k] = f ? 1u : 0u;
         }
     }
+    if (tid < K) pick[tid] = -1;
     __syncthreads();
-    const auto total = [&](int k, uint64_t key) {
+    const auto total = [&](int k, uint64_t key) -> uint64_t {
         return key == 0 ? 0ull : ordered64((double)score[k] + ((double)value_of((uint32_t)(key >> 32)) - lse[k]));
-    };
-    const auto before = [&](int i, int j) { return tot[i] > tot[j] || (tot[i] == tot[j] && tag[i] < tag[j]); };
-    const auto swap = [&](int i, int j) {
-        const uint64_t t = tot[i];
-        tot[i] = tot[j];
-        tot[j] = t;
-        const uint32_t g = tag[i];
-        tag[i] = tag[j];
-        tag[j] = g;
     };
     // heads of the K * C lists, tag = list; equal totals of one row's lists are ordered by index, as chunks are, and
     // those of different rows by row
-    int n = 1;
-    while (n < K * C) n <<= 1;
-    for (int i = tid; i < n; i += kJoinThreads) {
-        uint64_t t = 0;
-        if (i < K * C) {
-            const int k = i / C;
-            if (!fin[k]) t = total(k, A.lists[(base * C + i) * K]);
-            else if (i % C == 0) t = ordered64((double)score[k]);
-        }
-        tot[i] = t;
-        tag[i] = (uint32_t)i;
-    }
-    __syncthreads();
-    sort_shared<kJoinThreads>(n, before, swap);
-    if (tid < K) pick[tid] = tid < n && tot[tid] != 0 ? (int)tag[tid] : -1;
-    __syncthreads();
-    // all entries of those lists, tag = k * V + token
-    n = 1;
-    while (n < K * K) n <<= 1;
-    for (int i = tid; i < n; i += kJoinThreads) {
-        uint64_t t = 0;
-        uint32_t f = 0xFFFFFFFFu;
+    const auto head_of = [&](int i, uint64_t key) -> uint64_t {
+        const int k = i / C;
+        return !fin[k] ? total(k, key) : i % C == 0 ? ordered64((double)score[k]) : 0ull;
+    };
+    // entry i of the best lists, tag = k * V + token
+    const auto entry_of = [&](int i, uint32_t &f) -> uint64_t {
         const int list = i < K * K ? pick[i / K] : -1;
-        if (list >= 0) {
-            const int k = list / C;
-            if (!fin[k]) {
-                const uint64_t key = A.lists[(base * C + list) * K + i % K];
-                t = total(k, key);
-                f = (uint32_t)(k * A.V) + (0xFFFFFFFFu - (uint32_t)key);
-            } else if (i % K == 0) {
-                t = ordered64((double)score[k]);
-                f = (uint32_t)(k * A.V) + (uint32_t)A.eos;
-            }
+        f = 0xFFFFFFFFu;
+        if (list < 0) return 0;
+        const int k = list / C;
+        if (!fin[k]) {
+            const uint64_t key = A.lists[(base * C + list) * K + i % K];
+            f = (uint32_t)(k * A.V) + (0xFFFFFFFFu - (uint32_t)key);
+            return total(k, key);
         }
-        tot[i] = t;
-        tag[i] = f;
-    }
-    __syncthreads();
-    sort_shared<kJoinThreads>(n, before, swap);
-    if (tid < K) {
-        const uint64_t t = tot[tid];
-        const int k = t ? (int)(tag[tid] / (uint32_t)A.V) : tid;
-        const int64_t token = t ? (int64_t)(tag[tid] % (uint32_t)A.V) : -1;
-        A.scores_out[base + tid] = t ? (float)total_of(t) : -INFINITY;
-        A.parents[base + tid] = k;
-        A.tokens[base + tid] = token;
-        if (A.done_out != nullptr) A.done_out[base + tid] = t == 0 || fin[k] || token == A.eos ? 1 : 0;
+        f = (uint32_t)(k * A.V) + (uint32_t)A.eos;
+        return i % K == 0 ? ordered64((double)score[k]) : 0;
+    };
+    const auto write = [&](int i, uint64_t t, uint32_t f) {
+        const int k = t ? (int)(f / (uint32_t)A.V) : i;
+        const int64_t token = t ? (int64_t)(f % (uint32_t)A.V) : -1;
+        A.scores_out[base + i] = t ? (float)total_of(t) : -INFINITY;
+        A.parents[base + i] = k;
+        A.tokens[base + i] = token;
+        if (A.done_out != nullptr) A.done_out[base + i] = t == 0 || fin[k] || token == A.eos ? 1 : 0;
+    };
+    if constexpr (COUNT) {
+        // how many of the n cells come before (t, f); cells that are no candidates come after all others
+        const auto rank = [&](int n, uint64_t t, uint32_t f) {
+            int r = 0;
+            for (int j = 0; j < n; ++j) r += tot[j] > t || (tot[j] == t && tag[j] < f);
+            return r;
+        };
+        const uint64_t h = tid < K * C ? head_of(tid, head) : 0;
+        if (tid < K * C) {
+            tot[tid] = h;
+            tag[tid] = (uint32_t)tid;
+        }
+        __syncthreads();
+        if (h != 0) {
+            const int r = rank(K * C, h, (uint32_t)tid);
+            if (r < K) pick[r] = tid;
+        }
+        __syncthreads();
+        uint32_t f;
+        const uint64_t t = entry_of(tid, f);
+        if (tid < K * K) {
+            tot[tid] = t;
+            tag[tid] = f;
+        }
+        const int some = __syncthreads_count(t != 0);
+        if (t != 0) {
+            const int r = rank(K * K, t, f);
+            if (r < K) write(r, t, f);
+        }
+        if (tid < K && tid >= some) write(tid, 0, 0);
+    } else {
+        const auto before = [&](int i, int j) { return tot[i] > tot[j] || (tot[i] == tot[j] && tag[i] < tag[j]); };
+        const auto swap = [&](int i, int j) {
+            const uint64_t t = tot[i];
+            tot[i] = tot[j];
+            tot[j] = t;
+            const uint32_t g = tag[i];
+            tag[i] = tag[j];
+            tag[j] = g;
+        };
+        int n = 1;
+        while (n < K * C) n <<= 1;
+        for (int i = tid; i < n; i += THREADS) {
+            tot[i] = i < K * C ? head_of(i, A.lists[(base * C + i) * K]) : 0;
+            tag[i] = (uint32_t)i;
+        }
+        __syncthreads();
+        sort_shared<THREADS>(n, before, swap);
+        if (tid < K && tot[tid] != 0) pick[tid] = (int)tag[tid];
+        __syncthreads();
+        n = 1;
+        while (n < K * K) n <<= 1;
+        for (int i = tid; i < n; i += THREADS) {
+            uint32_t f;
+            const uint64_t t = entry_of(i, f);
+            tot[i] = t;
+            tag[i] = f;
+        }
+        __syncthreads();
+        sort_shared<THREADS>(n, before, swap);
+        if (tid < K) write(tid, tot[tid], tag[tid]);
     }
 }
 
@@ -328,10 +367,20 @@ int vgx_beam_select(const float *logits, int64_t ld, int64_t groups, int64_t K, 
     else
         hipLaunchKernelGGL((chunk_kernel<16>), grid, dim3(kThreads), 0, st, logits, ld, (int)V, (int)K, done, lists, sums);
     VGX_CHECK_LAUNCH();
-    int cells = 1;
-    while (cells < K * C || cells < K * K) cells <<= 1;
     const JoinArgs A{lists, sums, scores, done, scores_out, parents, tokens, done_out, eos, (int)V, (int)K, (int)C};
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)groups), dim3(kJoinThreads), (size_t)cells * 12, st, A, cells);
+    const int most = (int)std::max(K * C, K * K);
+    const auto join = [&](auto kernel, int threads, int cells) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(threads), (size_t)cells * 12, st, A, cells);
+    };
+    if (most <= kThreads) {
+        join(join_kernel<kThreads, true>, kThreads, most);
+    } else if (most <= kJoinThreads) {
+        join(join_kernel<kJoinThreads, true>, kJoinThreads, most);
+    } else {
+        int cells = 1;
+        while (cells < most) cells <<= 1;
+        join(join_kernel<kJoinThreads, false>, kJoinThreads, cells);
+    }
     VGX_CHECK_LAUNCH();
     return VGX_OK;
 }

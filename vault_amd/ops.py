@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 import sys
 from typing import Optional, Tuple
 
@@ -27,7 +28,12 @@ def payload_bytes(dtype: int, rows: int, cols: int) -> int:
     return rows * (cols // 32) * BLOCK_BYTES[dtype]
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # what current_stream() wraps, a tenth of its time
+
+
 def _stream(dev: torch.device) -> int:
+    if _raw_stream is not None and dev.index is not None:
+        return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
 
 
@@ -36,7 +42,12 @@ _HERE = contextlib.nullcontext()
 
 def _on(dev: torch.device):
     """A context in which ``dev`` is the current device (a launch goes to the current one, whatever its stream)."""
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE if _one_device() or torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+@functools.lru_cache(maxsize=1)
+def _one_device() -> bool:
+    return torch.cuda.device_count() == 1
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -798,26 +809,33 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: Optional[torch
         raise ValueError("logits must be [B * K, V] and scores [B, K]")
     if logits.stride(1) != 1 or not scores.is_contiguous():
         raise ValueError("logits rows and scores must be contiguous")
-    dev = logits.device
-    if scores.device != dev:
+    index = logits.get_device()
+    if scores.get_device() != index:
         raise ValueError("logits and scores must be on one device")
     if done is not None:
         _need(done, torch.uint8, "done")
-        if done.shape != scores.shape or not done.is_contiguous() or done.device != dev:
+        if done.shape != scores.shape or not done.is_contiguous() or done.get_device() != index:
             raise ValueError("done must be a contiguous uint8 tensor like scores")
         if eos < 0:
             raise ValueError("finished beams need eos")
-    (B, K), V = scores.shape, logits.shape[1]
-    lib = L.load()
-    need = int(lib.vgx_beam_select_workspace_bytes(B, K, V))
-    L.check(min(need, 0), "vgx_beam_select_workspace_bytes")
+    (B, K), V, dev = scores.shape, logits.shape[1], logits.device
+    need = _beam_bytes(B, K, V)
     buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=dev)
     out = torch.empty_like(scores)
     parents = torch.empty(B, K, dtype=torch.int32, device=dev)
     tokens = torch.empty(B, K, dtype=torch.int64, device=dev)
     done_out = torch.empty(B, K, dtype=torch.uint8, device=dev)
     with _on(dev):
-        L.check(lib.vgx_beam_select(logits.data_ptr(), logits.stride(0), B, K, V, scores.data_ptr(), _ptr(done), eos,
-                                    out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), done_out.data_ptr(),
-                                    buf.data_ptr(), buf.numel(), _stream(dev)), "vgx_beam_select")
+        rc = L.load().vgx_beam_select(logits.data_ptr(), logits.stride(0), B, K, V, scores.data_ptr(), _ptr(done), eos,
+                                      out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), done_out.data_ptr(),
+                                      buf.data_ptr(), buf.numel(), _stream(dev))
+    if rc:
+        L.check(rc, "vgx_beam_select")
     return out, parents, tokens, done_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _beam_bytes(B: int, K: int, V: int) -> int:
+    need = int(L.load().vgx_beam_select_workspace_bytes(B, K, V))
+    L.check(min(need, 0), "vgx_beam_select_workspace_bytes")
+    return need

@@ -14,6 +14,7 @@ outside the cache, lengths past the table) are not errors: see include/vault_amd
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -61,7 +62,9 @@ class PagedKV:
         self.device = k.device
         self._c = L.PagedKV(fmt, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, pages, G, P, D,
                             k.stride(0) if n > 1 else pages * G * P * D, k_scale.stride(0) if n > 1 else pages * G)
-        self._ref = C.addressof(self._c)
+        self.ref = C.addressof(self._c)
+        self.index = k.get_device()
+        self.lib = L.load()
 
     @classmethod
     def empty(cls, n_layers: int, n_pages: int, G: int, D: int, device, page: int = 64, fmt: int = I8) -> "PagedKV":
@@ -73,40 +76,58 @@ class PagedKV:
                    fmt)
 
 
-def _words(t: torch.Tensor, shape, dev, name: str) -> None:
-    if t.dtype != torch.int32 or t.device != dev:
+# A decode step makes these calls per layer and token, so the checks below are as cheap as Python allows: devices are
+# compared by index, and the launch context, the stream and the workspace's size cost no more than a dictionary look-up.
+
+def _words(t: torch.Tensor, n: int, kv: PagedKV, name: str) -> None:
+    if t.dtype is not torch.int32 or t.get_device() != kv.index:
         raise ValueError(f"{name} must be an int32 tensor on the cache's device")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must be [{n}], got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
 
-def _table(t: torch.Tensor, dev, name: str = "table") -> None:
-    if t.dtype != torch.int32 or t.device != dev or t.dim() != 2 or t.shape[1] < 1:
+def _table(t: torch.Tensor, kv: PagedKV, name: str = "table") -> Tuple[int, int, int]:
+    """(sequences, entries, row stride)."""
+    if t.dtype is not torch.int32 or t.get_device() != kv.index or t.dim() != 2:
         raise ValueError(f"{name} must be int32 [sequences, entries] on the cache's device")
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    B, n = t.shape
+    if n < 1:
+        raise ValueError(f"{name} must have entries")
+    if t.is_contiguous():
+        return B, n, n
+    ld = t.stride(0) if B > 1 else n
+    if t.stride(1) != 1 or ld < n:
         raise ValueError(f"{name} rows must be contiguous and apart")
+    return B, n, ld
 
 
-def _rows(t: torch.Tensor, heads: Optional[int], D: int, dtype, dev, name: str) -> torch.Tensor:
+def _aligned(t: torch.Tensor) -> bool:
+    """Whether [N, heads, D] has contiguous heads and 16-byte aligned rows."""
+    if t.data_ptr() % 16:
+        return False
+    if t.is_contiguous():
+        return True
+    N, H, D = t.shape
+    st = t.stride()
+    return st[2] == 1 and (H == 1 or st[1] == D) and (N == 1 or (st[0] * t.element_size() % 16 == 0 and st[0] >= H * D))
+
+
+def _rows(t: torch.Tensor, heads: Optional[int], dtype, kv: PagedKV, name: str) -> torch.Tensor:
     """[N, heads, D] with contiguous heads and 16-byte aligned rows (a copy where the view is not)."""
-    if t.dim() != 3 or t.shape[2] != D or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [N, {heads if heads is not None else 'H'}, {D}], got {tuple(t.shape)}")
-    if t.dtype != dtype or t.device != dev:
+    if t.dim() != 3 or t.shape[2] != kv.D or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [N, {heads if heads is not None else 'H'}, {kv.D}], got {tuple(t.shape)}")
+    if t.dtype is not dtype or t.get_device() != kv.index:
         raise ValueError(f"{name} must be {dtype} on the cache's device")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D) or t.data_ptr() % 16 or \
-            (t.shape[0] > 1 and (t.stride(0) * t.element_size() % 16 or t.stride(0) < t.shape[1] * D)):
-        return t.contiguous() if not t.is_contiguous() else t.clone()
-    return t
+    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _dest(t: torch.Tensor, like: torch.Tensor, name: str) -> None:
     """An output that rows are written into, in place."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+    if t.shape != like.shape or t.dtype is not like.dtype or t.get_device() != like.get_device():
         raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on the cache's device")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]) or t.data_ptr() % 16 or \
-            (t.shape[0] > 1 and (t.stride(0) * t.element_size() % 16 or t.stride(0) < t.shape[1] * t.shape[2])):
+    if not _aligned(t):
         raise ValueError(f"{name} needs contiguous heads and 16-byte aligned rows")
 
 
@@ -114,19 +135,24 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
-def _batch(table: torch.Tensor, q_start: Optional[torch.Tensor], N: int, dev) -> int:
-    B = table.shape[0]
+def _batch(q_start: Optional[torch.Tensor], B: int, N: int, kv: PagedKV) -> None:
     if q_start is None:
         if N != B:
             raise ValueError(f"without q_start every sequence has one row: {N} rows for {B} sequences")
     else:
-        _words(q_start, (B + 1,), dev, "q_start")
-    return B
+        _words(q_start, B + 1, kv, "q_start")
 
 
 def _layer(kv: PagedKV, layer: int) -> None:
     if not 0 <= layer < kv.n_layers:
         raise ValueError(f"layer {layer} of {kv.n_layers}")
+
+
+@functools.lru_cache(maxsize=1024)
+def _attn_bytes(*sizes: int) -> int:
+    need = int(L.load().vgx_paged_attn_workspace_bytes(*sizes))
+    L.check(min(need, 0), "vgx_paged_attn_workspace_bytes")
+    return need
 
 
 def append(kv: PagedKV, layer: int, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, *,
@@ -139,42 +165,44 @@ def append(kv: PagedKV, layer: int, k: torch.Tensor, v: torch.Tensor, table: tor
     row.  With q [N, H, D] (dtype of k) the queries are rotated too, into ``q_out`` (may be q; a new tensor by default),
     which is returned.  A sequence's pages must be in its table row; a page that is written must be in one row only.
     ``max_new`` is not needed and only accepted for symmetry with ``attend``."""
-    dev, G, D = kv.device, kv.G, kv.D
+    D = kv.D
     _layer(kv, layer)
-    _table(table, dev)
-    if k.dtype not in KV_DTYPES:
+    B, cols, ldt = _table(table, kv)
+    dt = KV_DTYPES.get(k.dtype)
+    if dt is None:
         raise ValueError("k must be fp32 or bf16")
-    k, v = _rows(k, G, D, k.dtype, dev, "k"), _rows(v, G, D, k.dtype, dev, "v")
+    k, v = _rows(k, kv.G, k.dtype, kv, "k"), _rows(v, kv.G, k.dtype, kv, "v")
     N = k.shape[0]
     if v.shape[0] != N:
         raise ValueError("k and v must have the same rows")
-    B = _batch(table, q_start, N, dev)
-    _words(start, (B,), dev, "start")
-    rope_ld = rope_rows = H = 0
+    _batch(q_start, B, N, kv)
+    _words(start, B, kv, "start")
+    rope_ld = rope_rows = H = ldq = ldqo = 0
     if rope is not None:
-        if rope.dtype != torch.float32 or rope.device != dev or rope.dim() != 2 or rope.shape[1] != D:
+        if rope.dtype is not torch.float32 or rope.get_device() != kv.index or rope.dim() != 2 or rope.shape[1] != D:
             raise ValueError("rope must be fp32 [positions, D] on the cache's device")
-        if rope.stride(1) != 1 or rope.stride(0) % 4 or rope.data_ptr() % 16:
-            raise ValueError("rope rows must be contiguous and 16-byte aligned")
         rope_ld, rope_rows = rope.stride(0), rope.shape[0]
+        if rope.stride(1) != 1 or rope_ld % 4 or rope_ld < D or rope.data_ptr() % 16:
+            raise ValueError("rope rows must be contiguous, apart and 16-byte aligned")
     src = None
     if q is not None:
-        src = _rows(q, None, D, k.dtype, dev, "q")
+        src = _rows(q, None, k.dtype, kv, "q")
         if src.shape[0] != N or src.shape[1] < 1:
             raise ValueError("q must have the rows of k")
         H = src.shape[1]
         if q_out is None:
-            q_out = torch.empty(N, H, D, dtype=k.dtype, device=dev)
+            q_out = torch.empty(N, H, D, dtype=k.dtype, device=kv.device)
         else:
             _dest(q_out, q, "q_out")
+        ldq, ldqo = _ld(src), _ld(q_out)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    with _on(dev):
-        L.check(L.load().vgx_paged_append(
-            kv._ref, layer, KV_DTYPES[k.dtype], k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), N, table.data_ptr(),
-            table.stride(0) if B > 1 else table.shape[1], table.shape[1], start.data_ptr(), _ptr(q_start), B, _ptr(rope),
-            rope_ld, rope_rows, _ptr(src), _ld(src) if src is not None else 0, _ptr(q_out),
-            _ld(q_out) if q_out is not None else 0, H, _stream(dev)), "vgx_paged_append")
+    with _on(kv.device):
+        rc = kv.lib.vgx_paged_append(kv.ref, layer, dt, k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), N, table.data_ptr(), ldt,
+                                     cols, start.data_ptr(), _ptr(q_start), B, _ptr(rope), rope_ld, rope_rows, _ptr(src), ldq,
+                                     _ptr(q_out), ldqo, H, _stream(kv.device))
+    if rc:
+        L.check(rc, "vgx_paged_append")
     return q_out
 
 
@@ -190,42 +218,42 @@ def attend(kv: PagedKV, layer: int, q: torch.Tensor, table: torch.Tensor, lens: 
     nothing gets zeros, rows behind the last sequence stay as they were.  ``max_new`` / ``max_keys``: the most rows and
     keys of one sequence, hints for the split of the work (by default what the shapes allow).  ``ws``: a Workspace of this
     stream; without it scratch is allocated."""
-    dev, G, D = kv.device, kv.G, kv.D
+    D = kv.D
     _layer(kv, layer)
-    _table(table, dev)
-    if q.dtype not in KV_DTYPES:
+    B, cols, ldt = _table(table, kv)
+    dt = KV_DTYPES.get(q.dtype)
+    if dt is None:
         raise ValueError("q must be fp32 or bf16")
-    src = _rows(q, None, D, q.dtype, dev, "q")
+    src = _rows(q, None, q.dtype, kv, "q")
     N, H = src.shape[0], src.shape[1]
-    if H < 1 or H % G:
-        raise ValueError(f"{H} query heads for {G} kv heads")
-    B = _batch(table, q_start, N, dev)
-    _words(lens, (B,), dev, "lens")
+    if H < 1 or H % kv.G:
+        raise ValueError(f"{H} query heads for {kv.G} kv heads")
+    _batch(q_start, B, N, kv)
+    _words(lens, B, kv, "lens")
     if window < 0 or n_sink < 0:
         raise ValueError("window and n_sink must not be negative")
     if out is None:
-        out = torch.empty(N, H, D, dtype=q.dtype, device=dev)
+        out = torch.empty(N, H, D, dtype=q.dtype, device=kv.device)
     else:
         _dest(out, q, "out")
     most = 1 if q_start is None else N if max_new is None else max_new
-    keys = table.shape[1] * kv.page
+    keys = cols * kv.page
     keys = keys if max_keys is None else min(max_keys, keys)
     if most < 0 or keys < 0:
         raise ValueError("max_new and max_keys must not be negative")
-    lib = L.load()
-    need = int(lib.vgx_paged_attn_workspace_bytes(N, B, H, G, D, most, keys, window, n_sink))
-    L.check(min(need, 0), "vgx_paged_attn_workspace_bytes")
+    need = _attn_bytes(N, B, H, kv.G, D, most, keys, window, n_sink)
     buf = None
     if need > 0:
-        buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=dev)
-        if buf.device != dev:
+        buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=kv.device)
+        if buf.get_device() != kv.index:
             raise ValueError("the workspace must be on the cache's device")
-    with _on(dev):
-        L.check(lib.vgx_paged_attn(
-            kv._ref, layer, KV_DTYPES[q.dtype], src.data_ptr(), _ld(src), out.data_ptr(), _ld(out), N, H,
-            table.data_ptr(), table.stride(0) if B > 1 else table.shape[1], table.shape[1], lens.data_ptr(),
-            _ptr(q_start), B, most, keys, window, n_sink, float(scale if scale is not None else D ** -0.5), _ptr(buf),
-            buf.numel() if buf is not None else 0, _stream(dev)), "vgx_paged_attn")
+        need = buf.numel()
+    with _on(kv.device):
+        rc = kv.lib.vgx_paged_attn(kv.ref, layer, dt, src.data_ptr(), _ld(src), out.data_ptr(), _ld(out), N, H,
+                                   table.data_ptr(), ldt, cols, lens.data_ptr(), _ptr(q_start), B, most, keys, window, n_sink,
+                                   D ** -0.5 if scale is None else scale, _ptr(buf), need, _stream(kv.device))
+    if rc:
+        L.check(rc, "vgx_paged_attn")
     return out
 
 
@@ -234,21 +262,21 @@ def read(kv: PagedKV, table: torch.Tensor, first: torch.Tensor, n: int, lens: to
     """Dequantized rows of all layers (vgx_paged_read): (k, v), each [layers, B, G, n, D] fp32 or bf16, row i of sequence
     b being position first[b] + i; zeros at positions below 0 or at or past lens[b], and where the table has no page.
     Keys come back rotated as they were stored."""
-    dev = kv.device
-    _table(table, dev)
-    B = table.shape[0]
-    _words(first, (B,), dev, "first")
-    _words(lens, (B,), dev, "lens")
-    if dtype not in KV_DTYPES:
+    B, cols, ldt = _table(table, kv)
+    _words(first, B, kv, "first")
+    _words(lens, B, kv, "lens")
+    dt = KV_DTYPES.get(dtype)
+    if dt is None:
         raise ValueError("dtype must be fp32 or bf16")
     if n < 0:
         raise ValueError("n must not be negative")
-    k = torch.empty(kv.n_layers, B, kv.G, n, kv.D, dtype=dtype, device=dev)
+    k = torch.empty(kv.n_layers, B, kv.G, n, kv.D, dtype=dtype, device=kv.device)
     v = torch.empty_like(k)
-    with _on(dev):
-        L.check(L.load().vgx_paged_read(
-            kv._ref, KV_DTYPES[dtype], table.data_ptr(), table.stride(0) if B > 1 else table.shape[1], table.shape[1],
-            first.data_ptr(), lens.data_ptr(), B, n, k.data_ptr(), v.data_ptr(), _stream(dev)), "vgx_paged_read")
+    with _on(kv.device):
+        rc = kv.lib.vgx_paged_read(kv.ref, dt, table.data_ptr(), ldt, cols, first.data_ptr(), lens.data_ptr(), B, n,
+                                   k.data_ptr(), v.data_ptr(), _stream(kv.device))
+    if rc:
+        L.check(rc, "vgx_paged_read")
     return k, v
 
 
@@ -260,21 +288,20 @@ def reorder(kv: PagedKV, table: torch.Tensor, lens: torch.Tensor, parents: torch
     become shared; the page that the next token goes to is owned by one beam before and after (give every beam its own
     before the call): the first child takes its parent's over, further children get copies in the pages of beams that
     nothing continues.  Entries past that page stay the row's own.  A page stays in use until no table names it."""
-    dev = kv.device
-    if parents.dim() != 2:
-        raise ValueError("parents must be int32 [groups, K]")
+    if parents.dim() != 2 or parents.dtype is not torch.int32 or parents.get_device() != kv.index or \
+            not parents.is_contiguous():
+        raise ValueError("parents must be contiguous int32 [groups, K] on the cache's device")
     B, K = parents.shape
-    _words(parents, (B, K), dev, "parents")
-    _table(table, dev)
-    _table(table_out, dev, "table_out")
-    if table.shape[0] != B * K or table_out.shape != table.shape:
+    n, cols, ldt = _table(table, kv)
+    _, cols_out, ldo = _table(table_out, kv, "table_out")
+    if n != B * K or table_out.shape[0] != n or cols_out != cols:
         raise ValueError("table and table_out must have a row per beam")
-    _words(lens, (B * K,), dev, "lens")
-    _words(lens_out, (B * K,), dev, "lens_out")
+    _words(lens, n, kv, "lens")
+    _words(lens_out, n, kv, "lens_out")
     if table_out.data_ptr() == table.data_ptr() or lens_out.data_ptr() == lens.data_ptr():
         raise ValueError("table_out and lens_out must be other tensors than table and lens")
-    with _on(dev):
-        L.check(L.load().vgx_paged_reorder(
-            kv._ref, table.data_ptr(), table.stride(0) if B * K > 1 else table.shape[1], table.shape[1], lens.data_ptr(),
-            parents.data_ptr(), B, K, table_out.data_ptr(), table_out.stride(0) if B * K > 1 else table.shape[1],
-            lens_out.data_ptr(), _stream(dev)), "vgx_paged_reorder")
+    with _on(kv.device):
+        rc = kv.lib.vgx_paged_reorder(kv.ref, table.data_ptr(), ldt, cols, lens.data_ptr(), parents.data_ptr(), B, K,
+                                      table_out.data_ptr(), ldo, lens_out.data_ptr(), _stream(kv.device))
+    if rc:
+        L.check(rc, "vgx_paged_reorder")
