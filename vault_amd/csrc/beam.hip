@@ -157,8 +157,11 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(const float *__restrict
         while (w < kWaves && at >= count[w]) at -= count[w++];
         if (w < kWaves) k = keys[w * kCap + at];
         int rank = 0;
-        for (int u = 0; u < kWaves; ++u)
-            for (int i = 0; i < count[u]; ++i) rank += keys[u * kCap + i] > k;
+        for (int u = 0; u < kWaves; ++u) {
+            const int m = count[u];
+#pragma unroll 8
+            for (int i = 0; i < m; ++i) rank += keys[u * kCap + i] > k;
+        }
         if (k != 0 && rank < K) out[rank] = k;
         if (tid < K && tid >= total) out[tid] = 0;
         return;
@@ -272,7 +275,12 @@ __global__ __launch_bounds__(THREADS) void join_kernel(const JoinArgs A, int cel
         // how many of the n cells come before (t, f); cells that are no candidates come after all others
         const auto rank = [&](int n, uint64_t t, uint32_t f) {
             int r = 0;
-            for (int j = 0; j < n; ++j) r += tot[j] > t || (tot[j] == t && tag[j] < f);
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) {
+                const uint64_t a = tot[j];
+                const uint32_t g = tag[j];
+                r += (int)(a > t) | ((int)(a == t) & (int)(g < f));
+            }
             return r;
         };
         const uint64_t h = tid < K * C ? head_of(tid, head) : 0;
