@@ -65,14 +65,12 @@ VGX_DEV void rotated8(const AppendArgs &A, int64_t row, int64_t pos, int g, int 
         for (int i = 0; i < 4; ++i) lo[i] = a[i], hi[i] = b[i];
         return;
     }
-    if (pos >= A.rope_rows) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lo[i] = hi[i] = NAN;
-        return;
+    const bool known = pos < A.rope_rows;
+    float c[4] = {NAN, NAN, NAN, NAN}, s[4] = {NAN, NAN, NAN, NAN};
+    if (known) {
+        load4<false>(A.rope, pos * A.rope_ld + d, c);
+        load4<false>(A.rope, pos * A.rope_ld + D / 2 + d, s);
     }
-    float c[4], s[4];
-    load4<false>(A.rope, pos * A.rope_ld + d, c);
-    load4<false>(A.rope, pos * A.rope_ld + D / 2 + d, s);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         lo[i] = (float)((double)a[i] * (double)c[i] - (double)b[i] * (double)s[i]);
@@ -126,57 +124,92 @@ VGX_DEV uint32_t again4(uint32_t w, const Scale &s) {
     return to_codes4<FMT>(c);
 }
 
-template <int FMT, int D, bool BF16>
-__global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs A) {
-    __shared__ uint32_t red[4];
-    extern __shared__ uint8_t tile[];            // V codes of the new tokens, [D][page]
-    const int tid = threadIdx.x;
-    if ((int64_t)blockIdx.x >= A.kv_groups) {
-        // queries: thread = eight dims of one head of one row
-        constexpr int T = D / 8;
-        const int64_t u = ((int64_t)blockIdx.x - A.kv_groups) * kThreads + tid;
-        const int64_t row = u / ((int64_t)A.H * T);
-        if (row >= A.N) return;
-        const int r = (int)(u - row * A.H * T), h = r / T, d = (r - h * T) * 4;
-        int b = (int)row;
-        int64_t pos = 0;
-        if (A.q_start != nullptr) {
-            int lo = 0, hi = A.B;                // the last b with q_start[b] <= row
-            if (row < A.q_start[0] || row >= A.q_start[A.B]) return;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (A.q_start[mid] <= row) lo = mid;
-                else hi = mid;
-            }
-            b = lo;
-            pos = row - A.q_start[b];
+// w[t] holds byte d of token t in its byte d; afterwards w[d] holds byte d of token t in its byte t.
+VGX_DEV void transpose_bytes(uint32_t (&w)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// Queries: a wave takes one row; a lane has 8 dims of the lower half of a head and their partners of the upper one, and
+// goes through the heads with its piece of the rotation in registers.
+template <int D, bool BF16>
+VGX_DEV void rotate_query(const AppendArgs &A, int64_t row) {
+    constexpr int T = D / 16, HEADS = 64 / T;
+    const int lane = threadIdx.x & 63, d = (lane % T) * 8;
+    int b = (int)row;
+    int64_t pos = 0;
+    if (A.q_start != nullptr) {
+        if (row < A.q_start[0] || row >= A.q_start[A.B]) return;
+        int lo = 0, hi = A.B;                    // the last b with q_start[b] <= row
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (A.q_start[mid] <= row) lo = mid;
+            else hi = mid;
         }
-        pos += A.start[b];
-        if (pos < 0) return;
-        float a[4], c[4], x[4], y[4];
-        load4<BF16>(A.q, row * A.ldq + (int64_t)h * D + d, a);
-        load4<BF16>(A.q, row * A.ldq + (int64_t)h * D + D / 2 + d, c);
-        if (A.rope == nullptr) {
+        b = lo;
+        pos = row - A.q_start[b];
+    }
+    pos += A.start[b];
+    if (pos < 0) return;
+    float cs[2][4], sn[2][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = a[i], y[i] = c[i];
-        } else if (pos >= A.rope_rows) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = y[i] = NAN;
-        } else {
-            float cs[4], sn[4];
-            load4<false>(A.rope, pos * A.rope_ld + d, cs);
-            load4<false>(A.rope, pos * A.rope_ld + D / 2 + d, sn);
+        for (int i = 0; i < 4; ++i) {
+            cs[j][i] = A.rope == nullptr ? 1.0f : NAN;
+            sn[j][i] = A.rope == nullptr ? 0.0f : NAN;
+        }
+    if (A.rope != nullptr && pos < A.rope_rows) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            load4<false>(A.rope, pos * A.rope_ld + d + 4 * j, cs[j]);
+            load4<false>(A.rope, pos * A.rope_ld + D / 2 + d + 4 * j, sn[j]);
+        }
+    }
+#pragma unroll 2
+    for (int h = lane / T; h < A.H; h += HEADS) {
+        const int64_t at = row * A.ldq + (int64_t)h * D + d, to = row * A.ldqo + (int64_t)h * D + d;
+        float a[2][4], c[2][4], x[2][4], y[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            load4<BF16>(A.q, at + 4 * j, a[j]);
+            load4<BF16>(A.q, at + D / 2 + 4 * j, c[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] = fmaf(a[i], cs[i], -(c[i] * sn[i]));
-                y[i] = fmaf(c[i], cs[i], a[i] * sn[i]);
+                x[j][i] = A.rope == nullptr ? a[j][i] : fmaf(a[j][i], cs[j][i], -(c[j][i] * sn[j][i]));
+                y[j][i] = A.rope == nullptr ? c[j][i] : fmaf(c[j][i], cs[j][i], a[j][i] * sn[j][i]);
             }
+            store4<BF16>(A.q_out, to + 4 * j, x[j]);
+            store4<BF16>(A.q_out, to + D / 2 + 4 * j, y[j]);
         }
-        store4<BF16>(A.q_out, row * A.ldqo + (int64_t)h * D + d, x);
-        store4<BF16>(A.q_out, row * A.ldqo + (int64_t)h * D + D / 2 + d, y);
+    }
+}
+
+// A workgroup stores the new tokens of one page and head: a thread has four tokens and, of each, four dims of the lower
+// half and their partners of the upper one.  ONCE: the page's tokens fit the workgroup's registers (64 of 128 dims), which
+// then hold them between the search for the largest magnitude and the rounding; otherwise they are read again.  V's codes
+// are turned from tokens to dims in registers, four by four, and pass through shared memory (rows of page + 4 bytes, so
+// that the dims of a wave's words lie in different banks) on their way to whole 16-byte pieces.  What bounds it is the
+// rotated queries' traffic: 13057 tokens of 32 / 8 heads in bf16, 223 MB, 63 us when every thread took two loads of its
+// rotation for 8 values of q and the tokens were read twice.
+template <int FMT, int D, bool BF16, bool ONCE>
+__global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs A) {
+    __shared__ uint32_t red[4];
+    extern __shared__ uint8_t tile[];
+    const int tid = threadIdx.x;
+    if ((int64_t)blockIdx.x >= A.kv_groups) {
+        const int64_t row = ((int64_t)blockIdx.x - A.kv_groups) * (kThreads / 64) + (tid >> 6);
+        if (row < A.N) rotate_query<D, BF16>(A, row);
         return;
     }
-    const int g = (int)(blockIdx.x % (unsigned)A.c.G), P = 1 << A.c.log_page;
+    const int g = (int)(blockIdx.x % (unsigned)A.c.G), P = 1 << A.c.log_page, S = P + 4;
     int64_t j = 0;
     const auto first_of = [&](int b, int &n) -> int64_t {      // first position at or above 0 and the tokens from it on
         const SeqRows r = seq_rows(A.q_start, b, A.N);
@@ -184,15 +217,20 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs A) {
         n = (int)max((int64_t)0, (int64_t)(r.hi - r.lo) - max((int64_t)0, -st));
         return max(st, (int64_t)0);
     };
-    const int b = find_unit((int64_t)blockIdx.x / A.c.G, A.B, [&](int i) {
-        int n;
-        const int64_t p = first_of(i, n);
-        return n <= 0 ? 0 : (int)(((p + n - 1) >> A.c.log_page) - (p >> A.c.log_page) + 1);
-    }, j);
-    if (b < 0) return;
+    int b = (int)(blockIdx.x / (unsigned)A.c.G);
+    if (A.q_start != nullptr) {
+        b = find_unit(b, A.B, [&](int i) {
+            int n;
+            const int64_t p = first_of(i, n);
+            return n <= 0 ? 0 : (int)(((p + n - 1) >> A.c.log_page) - (p >> A.c.log_page) + 1);
+        }, j);
+        b = __builtin_amdgcn_readfirstlane(b);
+        if (b < 0) return;
+    }
     int n;
     const int64_t p0 = first_of(b, n);
-    const int64_t col = (p0 >> A.c.log_page) + j;
+    if (n <= 0) return;
+    const int64_t col = (p0 >> A.c.log_page) + __builtin_amdgcn_readfirstlane((int)j);
     if (col >= A.cols) return;
     const int page = A.table[(int64_t)b * A.ldt + col];
     if (page < 0 || page >= A.c.n_pages) return;
@@ -204,22 +242,37 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs A) {
     const int64_t at = (int64_t)page * A.c.G + g, bytes = at * A.c.head_bytes;
     uint8_t *kp = A.c.k + bytes, *vp = A.c.v + bytes;
     const bool older = R.a > 0;
-    constexpr int T = D / 8;                                   // threads of one token
-    const int t = tid / T, d = (tid - t * T) * 4;
-
-    uint32_t kmax = 0, vmax = 0;
-    for (int i = R.a + t; i < R.z; i += kThreads / T) {
-        float x[4], y[4];
-        const int64_t row = R.row + (i - R.a);
-        rotated8<BF16, D>(A, row, R.pos0 + i, g, d, x, y);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) kmax = max(kmax, max(abs_bits(x[e]), abs_bits(y[e])));
-        load4<BF16>(A.v, row * A.ldv + (int64_t)g * D + d, x);
-        load4<BF16>(A.v, row * A.ldv + (int64_t)g * D + D / 2 + d, y);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vmax = max(vmax, max(abs_bits(x[e]), abs_bits(y[e])));
-    }
     const float was_k = A.c.ks[at], was_v = A.c.vs[at];
+    constexpr int T = D / 8, PER = 4 * kThreads / T;           // threads of a token, tokens of the workgroup
+    const int t4 = (tid / T) * 4, d = (tid % T) * 4;
+
+    float kx[4][2][4], vx[4][2][4];
+    const auto load = [&](int base) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int i = base + t4 + t;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) kx[t][0][e] = kx[t][1][e] = vx[t][0][e] = vx[t][1][e] = 0.0f;
+            if (i < R.a || i >= R.z) continue;
+            const int64_t row = R.row + (i - R.a);
+            rotated8<BF16, D>(A, row, R.pos0 + i, g, d, kx[t][0], kx[t][1]);
+            load4<BF16>(A.v, row * A.ldv + (int64_t)g * D + d, vx[t][0]);
+            load4<BF16>(A.v, row * A.ldv + (int64_t)g * D + D / 2 + d, vx[t][1]);
+        }
+    };
+    uint32_t kmax = 0, vmax = 0;
+    for (int base = R.a & ~3; base < R.z; base += PER) {
+        load(base);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    kmax = max(kmax, abs_bits(kx[t][h][e]));
+                    vmax = max(vmax, abs_bits(vx[t][h][e]));
+                }
+    }
     kmax = block_max(kmax, red);
     vmax = block_max(vmax, red);
     const Scale sk = new_scale<FMT>(kmax, was_k, older), sv = new_scale<FMT>(vmax, was_v, older);
@@ -228,33 +281,39 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs A) {
         A.c.vs[at] = sv.now;
     }
     const double ik = sk.now > 0.0f ? 1.0 / (double)sk.now : 0.0, iv = sv.now > 0.0f ? 1.0 / (double)sv.now : 0.0;
-    for (int i = R.a + t; i < R.z; i += kThreads / T) {
-        float x[4], y[4];
-        const int64_t row = R.row + (i - R.a);
-        rotated8<BF16, D>(A, row, R.pos0 + i, g, d, x, y);
-        quotients(x, ik);
-        quotients(y, ik);
-        *reinterpret_cast<uint32_t *>(kp + (int64_t)i * D + d) = to_codes4<FMT>(x);
-        *reinterpret_cast<uint32_t *>(kp + (int64_t)i * D + D / 2 + d) = to_codes4<FMT>(y);
-        load4<BF16>(A.v, row * A.ldv + (int64_t)g * D + d, x);
-        load4<BF16>(A.v, row * A.ldv + (int64_t)g * D + D / 2 + d, y);
-        quotients(x, iv);
-        quotients(y, iv);
-        const uint32_t lo = to_codes4<FMT>(x), hi = to_codes4<FMT>(y);
+    for (int base = R.a & ~3; base < R.z; base += PER) {
+        if (!ONCE) load(base);
+        if (base + t4 >= R.z) continue;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            tile[(d + e) * P + i] = (uint8_t)(lo >> (8 * e));
-            tile[(d + D / 2 + e) * P + i] = (uint8_t)(hi >> (8 * e));
+        for (int h = 0; h < 2; ++h) {
+            uint32_t w[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int i = base + t4 + t;
+                quotients(kx[t][h], ik);
+                if (i >= R.a && i < R.z)
+                    *reinterpret_cast<uint32_t *>(kp + (int64_t)i * D + h * (D / 2) + d) = to_codes4<FMT>(kx[t][h]);
+                quotients(vx[t][h], iv);
+                w[t] = to_codes4<FMT>(vx[t][h]);
+            }
+            transpose_bytes(w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint32_t *>(tile + (h * (D / 2) + d + e) * S + base + t4) = w[e];
         }
     }
     __syncthreads();
     // V rows are dims: whole 16-byte pieces of new tokens at once, the ends of the run byte by byte
-    for (int u = tid; u < D * P / 16; u += kThreads) {
-        const int dim = u / (P / 16), i0 = (u - dim * (P / 16)) * 16, o = dim * P + i0;
+    const int c0 = R.a / 16, cn = (R.z + 15) / 16 - c0;        // the 16-token pieces that the run touches
+    for (int u = tid; u < D * cn; u += kThreads) {
+        const int dim = u / cn, i0 = (c0 + u - dim * cn) * 16;
+        const uint8_t *src = tile + dim * S + i0;
+        uint8_t *dst = vp + dim * P + i0;
         if (i0 >= R.a && i0 + 16 <= R.z) {
-            *reinterpret_cast<uint4 *>(vp + o) = *reinterpret_cast<const uint4 *>(tile + o);
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(src);
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
-            for (int i = max(i0, R.a); i < min(i0 + 16, R.z); ++i) vp[dim * P + i] = tile[dim * P + i];
+            for (int i = max(i0, R.a) - i0; i < min(i0 + 16, R.z) - i0; ++i) dst[i] = src[i];
         }
     }
     if (sk.grown)
@@ -269,48 +328,65 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs A) {
         }
 }
 
-// One page of one (layer, sequence, head): K rows as they lie, V through shared memory.
+// One page of one (layer, sequence, head).  A thread has four tokens of four dims: K's words lie that way, V's are words
+// of four tokens and pass through shared memory (rows of page + 4 bytes: with rows of a page of 128 the dims of a wave
+// shared one bank, 335 us for 128 such pages of 28 layers, 1.2 GB).
 template <int FMT, int D, bool BF16>
 __global__ __launch_bounds__(kThreads) void read_kernel(const vgx_paged_kv kv, int log_page, const int32_t *table,
                                                         int64_t ldt, int cols, const int32_t *first,
                                                         const int32_t *lens, int n, void *k_out, void *v_out) {
     extern __shared__ uint8_t tile[];
-    const int tid = threadIdx.x, P = 1 << log_page, G = (int)kv.G;
+    const int tid = threadIdx.x, P = 1 << log_page, S = P + 4, G = (int)kv.G;
     const int g = (int)(blockIdx.y % (unsigned)G), b = (int)(blockIdx.y / (unsigned)G), layer = blockIdx.z;
-    const int64_t f = first[b], col = (f >> log_page) + blockIdx.x, p0 = col << log_page;
+    const int64_t f = first[b], len = lens[b], col = (f >> log_page) + blockIdx.x, p0 = col << log_page;
     const int lo = (int)max((int64_t)0, f - p0), hi = (int)min((int64_t)P, f + n - p0);   // the page's tokens to write
     if (hi <= lo) return;
     const int page = col >= 0 && col < cols ? table[(int64_t)b * ldt + col] : -1;
     const bool have = page >= 0 && page < kv.n_pages;
-    const int end = have ? (int)min((int64_t)hi, (int64_t)lens[b] - p0) : 0;               // tokens below it exist
+    const int end = have ? (int)max((int64_t)0, min((int64_t)hi, len - p0)) : 0;                            // tokens below it exist
     const int64_t at = (int64_t)max(page, 0) * G + g, bytes = layer * kv.layer_stride + at * (P * D);
     const int64_t row0 = (((int64_t)layer * (gridDim.y / (unsigned)G) + b) * G + g) * n + (p0 - f);
     float ks = 0.0f, vs = 0.0f;
     if (end > lo) {
         ks = kv.k_scale[layer * kv.scale_layer_stride + at];
         vs = kv.v_scale[layer * kv.scale_layer_stride + at];
-        for (int u = tid; u < D * P / 16; u += kThreads)
-            reinterpret_cast<uint4 *>(tile)[u] = reinterpret_cast<const uint4 *>(kv.v + bytes)[u];
+        const int c0 = lo / 16, cn = (end + 15) / 16 - c0;     // the 16-token pieces asked for
+        for (int u = tid; u < D * cn; u += kThreads) {
+            const int dim = u / cn, i0 = (c0 + u - dim * cn) * 16;
+            const uint4 w = *reinterpret_cast<const uint4 *>(kv.v + bytes + dim * P + i0);
+            uint32_t *t = reinterpret_cast<uint32_t *>(tile + dim * S + i0);
+            t[0] = w.x, t[1] = w.y, t[2] = w.z, t[3] = w.w;
+        }
     }
     __syncthreads();
     constexpr int T = D / 4;
     const int d = (tid % T) * 4;
-    for (int i = lo + tid / T; i < hi; i += kThreads / T) {
-        float x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
-        if (i < end) {
-            code_values4<FMT>(*reinterpret_cast<const uint32_t *>(kv.k + bytes + (int64_t)i * D + d), x);
+    for (int i0 = (lo & ~3) + tid / T * 4; i0 < hi; i0 += kThreads / T * 4) {
+        uint32_t kw[4], vw[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] *= ks;
-                y[e] = code_value<FMT>(tile[(d + e) * P + i]) * vs;
+        for (int t = 0; t < 4; ++t)                            // the page's tokens, whether asked for or not
+            kw[t] = i0 < end ? *reinterpret_cast<const uint32_t *>(kv.k + bytes + (int64_t)(i0 + t) * D + d) : 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vw[e] = i0 < end ? *reinterpret_cast<const uint32_t *>(tile + (d + e) * S + i0) : 0u;
+        transpose_bytes(vw);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int i = i0 + t;
+            if (i < lo || i >= hi) continue;
+            float x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
+            if (i < end) {
+                code_values4<FMT>(kw[t], x);
+                code_values4<FMT>(vw[t], y);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] *= ks, y[e] *= vs;
             }
+            store4<BF16>(k_out, (row0 + i) * D + d, x);
+            store4<BF16>(v_out, (row0 + i) * D + d, y);
         }
-        store4<BF16>(k_out, (row0 + i) * D + d, x);
-        store4<BF16>(v_out, (row0 + i) * D + d, y);
     }
 }
 
-// Workgroup (beam, layer); those of one extra layer write the tables.  Every wave works out the group's heirs from the
+// Workgroup (beam, layer, slice of the page); those of one extra layer write the tables.  Every wave works out the group's heirs from the
 // parents: lane i is beam i.
 __global__ __launch_bounds__(kThreads) void reorder_kernel(const vgx_paged_kv kv, int log_page, const int32_t *table,
                                                            int64_t ldt, int cols, const int32_t *lens,
@@ -342,6 +418,7 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(const vgx_paged_kv kv
     const int64_t at = (int64_t)len >> log_page, give_at = (int64_t)max(lens[grow], 0) >> log_page;
     const int dst = give_at < cols ? table[grow * ldt + give_at] : -1;
     if (blockIdx.y == kv.n_layers) {
+        if (blockIdx.z != 0) return;
         const int64_t mine = (int64_t)max(lens[row], 0) >> log_page;
         for (int64_t j = tid; j < cols; j += kThreads)
             table_out[row * ldt_out + j] = j < at ? table[prow * ldt + j]
@@ -359,10 +436,15 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(const vgx_paged_kv kv
     const auto *vs = reinterpret_cast<const uint4 *>(kv.v + lo + src * page_bytes);
     auto *kd = reinterpret_cast<uint4 *>(kv.k + lo + dst * page_bytes);
     auto *vd = reinterpret_cast<uint4 *>(kv.v + lo + dst * page_bytes);
-    for (int64_t u = tid; u < page_bytes / 16; u += kThreads) {
-        kd[u] = ks[u];
-        vd[u] = vs[u];
+    const int64_t pieces = page_bytes / 16, per = (pieces + gridDim.z - 1) / gridDim.z;
+    const int64_t u1 = min(pieces, (blockIdx.z + 1) * per);
+#pragma unroll 2
+    for (int64_t u = blockIdx.z * per + tid; u < u1; u += kThreads) {
+        const uint4 a = ks[u], c = vs[u];
+        kd[u] = a;
+        vd[u] = c;
     }
+    if (blockIdx.z != 0) return;
     for (int64_t g = tid; g < kv.G; g += kThreads) {
         kv.k_scale[s0 + dst * kv.G + g] = kv.k_scale[s0 + src * kv.G + g];
         kv.v_scale[s0 + dst * kv.G + g] = kv.v_scale[s0 + src * kv.G + g];
@@ -407,12 +489,16 @@ int vgx_paged_append(const vgx_paged_kv *kv, int64_t layer, int dtype, const voi
     // a sequence's n rows touch at most n / page + 2 pages, and no more than n
     const int64_t slots = q_start ? std::min(N, N / kv->page + 2 * B) : B;
     A.kv_groups = slots * kv->G;
-    const int64_t q_threads = q ? N * H * (kv->D / 8) : 0;
-    const int64_t groups = A.kv_groups + (q_threads + kThreads - 1) / kThreads;
+    const int64_t groups = A.kv_groups + (q ? (N + 3) / 4 : 0);
     if (groups > 0x7FFFFFFF) return VGX_E_LIMIT;
     return with_format(kv->fmt, kv->D, dtype == VGX_BF16, [&](auto fm, auto dm, auto bf) -> int {
-        hipLaunchKernelGGL((append_kernel<fm.value, dm.value, bf.value>), dim3((unsigned)groups), dim3(kThreads),
-                           (size_t)(kv->D * kv->page), (hipStream_t)stream, A);
+        const auto run = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kThreads), (size_t)(kv->D * (kv->page + 4)),
+                               (hipStream_t)stream, A);
+        };
+        // tokens that a workgroup holds at once
+        if (kv->page <= 4 * kThreads / (dm.value / 8)) run(append_kernel<fm.value, dm.value, bf.value, true>);
+        else run(append_kernel<fm.value, dm.value, bf.value, false>);
         VGX_CHECK_LAUNCH();
         return VGX_OK;
     });
@@ -434,7 +520,7 @@ int vgx_paged_read(const vgx_paged_kv *kv, int dtype, const int32_t *table, int6
     return with_format(kv->fmt, kv->D, dtype == VGX_BF16, [&](auto fm, auto dm, auto bf) -> int {
         hipLaunchKernelGGL((read_kernel<fm.value, dm.value, bf.value>),
                            dim3(pages, (unsigned)(B * kv->G), (unsigned)kv->n_layers), dim3(kThreads),
-                           (size_t)(kv->D * kv->page), (hipStream_t)stream, *kv, log_page, table, ldt, (int)table_cols,
+                           (size_t)(kv->D * (kv->page + 4)), (hipStream_t)stream, *kv, log_page, table, ldt, (int)table_cols,
                            first, lens, (int)n, k_out, v_out);
         VGX_CHECK_LAUNCH();
         return VGX_OK;
@@ -453,7 +539,9 @@ int vgx_paged_reorder(const vgx_paged_kv *kv, const int32_t *table, int64_t ldt,
     if (!lens || !parents || !lens_out || table_out == table || lens_out == lens) return VGX_E_ARG;
     if (groups * K > 0x7FFFFFFF || kv->n_layers >= 65535) return VGX_E_LIMIT;
     const int log_page = paged_layer(kv, 0).log_page;
-    hipLaunchKernelGGL(reorder_kernel, dim3((unsigned)(groups * K), (unsigned)kv->n_layers + 1), dim3(kThreads), 0,
+    // 16 KB of K and of V to a workgroup
+    const unsigned slices = (unsigned)std::min<int64_t>(16, std::max<int64_t>(1, kv->G * kv->page * kv->D / 16384));
+    hipLaunchKernelGGL(reorder_kernel, dim3((unsigned)(groups * K), (unsigned)kv->n_layers + 1, slices), dim3(kThreads), 0,
                        (hipStream_t)stream, *kv, log_page, table, ldt, (int)table_cols, lens, parents, (int)K, table_out,
                        ldt_out, lens_out);
     VGX_CHECK_LAUNCH();
