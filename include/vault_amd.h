@@ -360,6 +360,16 @@ int vgx_paged_attn(const vgx_paged_kv *kv, int64_t layer, int dtype, const void 
                    const int32_t *q_start, int64_t B, int64_t max_new, int64_t max_keys, int64_t window, int64_t n_sink,
                    float scale, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* vgx_paged_attn whose splits of few query rows are joined by the workgroup that finishes last instead of a second launch:
+ * tickets are n_tickets device int32, zero before the first call, which every call leaves at zero (calls sharing them must
+ * not overlap in time); with less than one for every kv head and (at most N * H / G / 16 + B) row tiles it runs as
+ * vgx_paged_attn.  The same bits. */
+int vgx_paged_attn_tickets(const vgx_paged_kv *kv, int64_t layer, int dtype, const void *q, int64_t ldq, void *out,
+                           int64_t ldo, int64_t N, int64_t H, const int32_t *table, int64_t ldt, int64_t table_cols,
+                           const int32_t *lens, const int32_t *q_start, int64_t B, int64_t max_new, int64_t max_keys,
+                           int64_t window, int64_t n_sink, float scale, void *workspace, int64_t workspace_bytes,
+                           int32_t *tickets, int64_t n_tickets, void *stream);
+
 /* Dequantized rows of every layer: k_out / v_out [n_layers][B][G][n][D] (dtype VGX_F32 or VGX_BF16; 16-byte aligned)
  * receive positions [first[b], first[b] + n) of sequence b (first, lens: device int32); zeros at positions below 0, at
  * or past lens[b], or without a page.  Brings a sequence back to the dense runs of vgx_attn_decode / vgx_attn_prefill. */

@@ -631,3 +631,56 @@ def test_two_streams(dev):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_attend_joined_in_the_launch(dev, fmt, dt):
+    """Splits joined by the last workgroup (a Workspace) give the bits of the joining launch (none); calls of several
+    batches share the workspace, whose tickets are zero after each; beam selection may use it in between."""
+    rng = np.random.default_rng(31)
+    ws = ops.Workspace(dev)
+    for lens, counts, H, D, P, G in (([3000], [1], 12, 128, 64, 2), ([2500, 70, 1], [1, 1, 1], 4, 64, 16, 4),
+                                     ([1500, 900], [3, 4], 8, 128, 32, 2), ([5000] * 3, [1] * 3, 32, 128, 128, 1)):
+        pages = sum(-(-n // P) for n in lens) + 2
+        c = _garbage(rng, pages, G, P, D, fmt)
+        table = _table(rng, lens, P, pages)
+        _fill(rng, c, table, lens)
+        kv = _to(c, dev)
+        q = torch.from_numpy(rng.standard_normal((sum(counts), H, D)).astype(np.float32)).to(DT[dt]).to(dev)
+        qs = None if set(counts) == {1} else _starts(counts, dev)
+        args = (kv, 1, q, _i32(table, dev), _i32(lens, dev))
+        kw = dict(q_start=qs, max_new=max(counts))
+        want = paged.attend(*args, **kw)
+        for _ in range(5):
+            assert torch.equal(paged.attend(*args, ws=ws, **kw), want)
+            assert not ws.tickets().any()
+        ops.beam_select(torch.randn(6, 9000, device=dev), torch.zeros(2, 3, device=dev), ws=ws)
+        out, size, reach, seen = op.attend(c, q.float().cpu().numpy(), table, lens, counts)
+        tol = op.attend_bound(out, size, reach, seen, D, dt == "bf16")
+        assert (np.abs(want.double().cpu().numpy() - out) <= tol).all()
+
+
+def test_captured_splits(dev):
+    """A captured call over several splits, replayed while the lengths grow and shrink, eager calls on the same workspace
+    in between (never at the same time)."""
+    rng = np.random.default_rng(32)
+    D, P, G, H = 128, 64, 2, 12
+    c = _garbage(rng, 80, G, P, D, "i8")
+    table = _table(rng, [4000], P, 80)
+    _fill(rng, c, table, [4000])
+    kv, t, lens = _to(c, dev), _i32(table, dev), _i32([4000], dev)
+    q, ws = torch.randn(1, H, D, device=dev), ops.Workspace(dev)
+    paged.attend(kv, 1, q, t, lens, ws=ws)
+    graph = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=s):
+        out = paged.attend(kv, 1, q, t, lens, ws=ws)
+    for n in (4000, 1, 0, 257, 64, 3999, 2000):
+        lens.fill_(n)
+        q.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, paged.attend(kv, 1, q, t, lens, ws=ws)) and torch.equal(got, paged.attend(kv, 1, q, t, lens))
+        assert not ws.tickets().any() and (n > 0 or not got.any())

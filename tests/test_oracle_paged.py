@@ -198,3 +198,12 @@ def test_refused_selections():
         assert lib.vgx_beam_select(*dict(base, **kw).values(), None) == code, kw
     assert lib.vgx_beam_select(*dict(base, groups=0).values(), None) == 0
     assert lib.vgx_beam_select_workspace_bytes(1, 0, 5) == -1
+
+
+def test_refused_tickets():
+    lib, kv = L.load(), _kv()
+    base = dict(layer=0, dtype=L.F32, q=p, ldq=1536, out=p, ldo=1536, N=3, H=12, table=p, ldt=4, cols=4, lens=p, q_start=p,
+                B=2, max_new=2, max_keys=256, window=0, n_sink=0, scale=1.0, ws=p, ws_bytes=1 << 30, tickets=p, n=64)
+    for kw, code in [(dict(n=-1), -1), (dict(tickets=p + 2), -11), (dict(out=None), -31), (dict(H=13), -7), (dict(ldq=1), -1)]:
+        assert lib.vgx_paged_attn_tickets(C.byref(kv), *dict(base, **kw).values(), None) == code, kw
+    assert lib.vgx_paged_attn_tickets(C.byref(kv), *dict(base, N=0).values(), None) == 0

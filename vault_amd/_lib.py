@@ -98,6 +98,8 @@ _SIGS = {
     "vgx_paged_attn_workspace_bytes": (I64, [I64, I64, I64, I64, I64, I64, I64, I64, I64]),
     "vgx_paged_attn": (I32, [P, I64, I32, P, I64, P, I64, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, F, P, I64,
                              P]),
+    "vgx_paged_attn_tickets": (I32, [P, I64, I32, P, I64, P, I64, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, F, P,
+                                     I64, P, I64, P]),
     "vgx_paged_read": (I32, [P, I32, P, I64, I64, P, P, I64, I64, P, P, P]),
     "vgx_paged_reorder": (I32, [P, P, I64, I64, P, P, I64, I64, P, I64, P, P]),
     "vgx_beam_select_workspace_bytes": (I64, [I64, I64, I64]),

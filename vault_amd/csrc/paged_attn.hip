@@ -39,7 +39,8 @@ struct AttnArgs {
     const int32_t *table, *lens, *q_start;
     float *part;
     float scale;
-    int N, B, H, R, cols, window, n_sink, splits, min_tiles;
+    int32_t *tickets;            // one per row tile and head, zero between calls; NULL: a launch of its own merges
+    int N, B, H, R, cols, window, n_sink, splits, per;
 };
 
 // RT query rows r0 .. of sequence b: row r is token r / R, head r % R of the group.
@@ -209,7 +210,7 @@ struct Entries {
 template <bool ONE>
 VGX_DEV Entries entries_of(const AttnArgs &A, const int32_t *__restrict__ row, int tok0) {
     // past the table: its last entry, for tokens that no row sees
-    const auto entry = [&](int tok) { return row[min(tok >> A.c.log_page, A.cols - 1)]; };
+    const auto entry = [&](int tok) { return row[min((int)((uint32_t)tok >> A.c.log_page), A.cols - 1)]; };
     if constexpr (ONE) {
         const int e = entry(tok0 + lane_zero());
         return {e, e};
@@ -265,13 +266,10 @@ struct Query {
     int last, from;
 };
 template <int D, bool BF16>
-VGX_DEV void load_query(const AttnArgs &A, const RowTile &rt, int g, int r, int last, Query<D, BF16 ? 1 : 2> &q) {
+VGX_DEV void load_query(const AttnArgs &A, const RowTile &rt, int g, int r, Query<D, BF16 ? 1 : 2> &q) {
     constexpr int KS = D / 32;
     const int grp = (threadIdx.x & 63) >> 4;
     const bool live = r < rt.r0 + rt.rows;
-    const int p = rt.len - rt.n + r / A.R;
-    q.last = live ? min(p, last) : -1;
-    q.from = A.window > 0 && live ? p - A.window : -1;
     float y[KS][8], most = 0.0f;
     const int64_t at = (int64_t)(rt.lo + (live ? r / A.R : 0)) * A.ldq + (int64_t)(g * A.R + (live ? r % A.R : 0)) * D;
 #pragma unroll
@@ -290,6 +288,13 @@ VGX_DEV void load_query(const AttnArgs &A, const RowTile &rt, int g, int r, int 
         pieces8<BF16 ? 1 : 2>(y[i], q.f[i]);
     }
     q.unit = ldexpf(fabsf(A.scale) * kLog2e, ex - kPre);
+}
+template <int D, int PIECES>
+VGX_DEV void see(const AttnArgs &A, const RowTile &rt, int r, int last, Query<D, PIECES> &q) {
+    const bool live = r < rt.r0 + rt.rows;
+    const int p = rt.len - rt.n + r / A.R;
+    q.last = live ? min(p, last) : -1;
+    q.from = A.window > 0 && live ? p - A.window : -1;
 }
 
 // Which of the 16 tokens from tok a row sees that sees those up to `last` after `from` and those below n_sink.
@@ -373,13 +378,14 @@ VGX_DEV void probabilities(const f32x4_t (&s)[4], uint32_t vis, float ks, float 
     }
 }
 
-// The range of key tiles of a split, and how many splits have any (one at least).
+// The key tiles of a split, `per` of them, whatever the sequence's length, so that the first one is known before the length
+// is (the last split takes what a hint too small leaves); and how many splits have any (one at least).
 struct Range {
     int first, end, used;
 };
 VGX_DEV Range range_of(const AttnArgs &A, int count, int split) {
-    const int per = max(A.min_tiles, (count + A.splits - 1) / A.splits);
-    return {split * per, min(count, (split + 1) * per), max(1, (count + per - 1) / per)};
+    const int used = min(A.splits, max(1, (count + A.per - 1) / A.per));
+    return {split * A.per, split == A.splits - 1 ? count : min(count, (split + 1) * A.per), used};
 }
 
 template <bool BF16>
@@ -397,34 +403,104 @@ VGX_DEV int64_t out_at(const AttnArgs &A, const RowTile &rt, int g, int row, int
     return (int64_t)(rt.lo + r / A.R) * A.ldo + (int64_t)(g * A.R + r % A.R) * D;
 }
 
+// Two floats of a partial state, written to and read from the level that all dies of the GPU share: a workgroup on one of
+// them joins what others wrote, within one launch (ordered by the ticket; a fence would write back a whole cache).
+VGX_DEV void put2(float *p, float a, float b) {
+    const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool SHARED>
+VGX_DEV float2 get2(const float *p) {
+    if constexpr (!SHARED) return *reinterpret_cast<const float2 *>(p);
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// Row rr of a tile of RT rows from its splits' partial states, by the 16 threads that ask for it: all loads of eight
+// splits at once.
+template <int RT, int D, bool BF16, bool SHARED>
+VGX_DEV void join_rows(const AttnArgs &A, const RowTile &rt, int64_t x, int g, int used, int rr) {
+    constexpr int V = D / 32;                        // pairs of floats of a thread
+    const int d = (threadIdx.x & 15) * 2;
+    if (rr >= rt.rows) return;
+    const int64_t step = (int64_t)RT * (D + 4);
+    const float *pp = A.part + (x * A.c.G + g) * A.splits * step + (int64_t)rr * (D + 4);
+    float M = kNeg, L = 0.0f, o[V][2] = {};
+    for (int s0 = 0; s0 < used; s0 += 8) {
+        float2 ml[8], v[8][V];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float *w = pp + min(s0 + u, used - 1) * step;
+            ml[u] = get2<SHARED>(w + D);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[u][j] = get2<SHARED>(w + j * 32 + d);
+        }
+        float now = M;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) now = fmaxf(now, ml[u].x);
+        const float f0 = __builtin_amdgcn_exp2f(M - now);
+        M = now;
+        L *= f0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j][0] *= f0, o[j][1] *= f0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float f = s0 + u < used ? __builtin_amdgcn_exp2f(ml[u].x - M) : 0.0f;
+            L = fmaf(f, ml[u].y, L);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                o[j][0] = fmaf(f, v[u][j].x, o[j][0]);
+                o[j][1] = fmaf(f, v[u][j].y, o[j][1]);
+            }
+        }
+    }
+    const int64_t at = out_at(A, rt, g, rr, D) + d;
+    const float inv = inverse(L);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if constexpr (BF16)
+            *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(A.out) + at + j * 32) = pack_bf16x2(o[j][0] * inv, o[j][1] * inv);
+        else
+            *reinterpret_cast<float2 *>(static_cast<float *>(A.out) + at + j * 32) = make_float2(o[j][0] * inv, o[j][1] * inv);
+    }
+}
+
 // One workgroup: a tile of 16 rows, a kv head and a range of its key tiles, dealt to the waves in turn.  For few query
 // rows per sequence: codes go from memory to registers of the one wave that multiplies them.
 template <int FMT, int D, bool BF16, bool ONE>
 __global__ __launch_bounds__(kThreads) void rows_kernel(const AttnArgs A) {
     constexpr int PIECES = BF16 ? 1 : 2, KS = D / 32, DT = D / 16, LD = D / 64;
     __shared__ float sm_m[kWaves][16], sm_l[kWaves][16], sm_o[kWaves][16][D + 4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15,
+              grp = lane >> 4;
     const int64_t x = blockIdx.x / (unsigned)A.c.G;
     const int g = (int)(blockIdx.x % (unsigned)A.c.G), split = blockIdx.y;
     const RowTile rt = row_tile<16>(A, x);
     if (rt.b < 0) return;
+    const int32_t *__restrict__ row = A.table + (int64_t)rt.b * A.ldt;
+    // what does not wait for the sequence's length: without a window the first tile's table entries, and the query
+    Entries ids{-1, -1};
+    if (A.window <= 0) ids = entries_of<ONE>(A, row, (split * A.per + wave) * kTile);
+    Query<D, PIECES> q;
+    load_query<D, BF16>(A, rt, g, rt.r0 + col, q);
     const int p0 = rt.len - rt.n;                                       // the position of the sequence's first query
     const int p_min = p0 + rt.r0 / A.R, p_max = p0 + (rt.r0 + rt.rows - 1) / A.R;
     const Tiles T = visible_tiles(A, p_min, p_max);
     const Range R = range_of(A, T.count, split);
     if (split >= R.used) return;
-    Query<D, PIECES> q;
-    load_query<D, BF16>(A, rt, g, rt.r0 + col, T.last, q);
+    see(A, rt, rt.r0 + col, T.last, q);
+    const auto token_of = [&](int ti) { return (ti < T.sinks ? ti : T.lo + ti - T.sinks) * kTile; };
+    if (A.window > 0 && R.first + wave < R.end) ids = entries_of<ONE>(A, row, token_of(R.first + wave));
 
-    const int32_t *__restrict__ row = A.table + (int64_t)rt.b * A.ldt;
     f32x4_t acc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) acc[i] = f32x4_t{0, 0, 0, 0};
     float m = kNeg, l = 0.0f;
 
     for (int ti = R.first + wave; ti < R.end; ti += kWaves) {
-        const int tok0 = (ti < T.sinks ? ti : T.lo + ti - T.sinks) * kTile;
-        const Pages<ONE> pg = pages_of<ONE>(A, entries_of<ONE>(A, row, tok0));
+        const int tok0 = token_of(ti);
+        const Pages<ONE> pg = pages_of<ONE>(A, ids);
+        if (ti + kWaves < R.end) ids = entries_of<ONE>(A, row, token_of(ti + kWaves));
         const float ks = A.c.ks[(int64_t)pg.v * A.c.G + g], vs = A.c.vs[(int64_t)pg.v * A.c.G + g];
         uint4 kw[4][LD], vw[DT];
         const uint8_t *kp = k_rows<ONE, D>(A, pg, g, tok0, 0), *vp = v_rows<ONE>(A, pg, g, tok0, 0);
@@ -513,12 +589,29 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const AttnArgs A) {
         }
         if (R.used > 1) {
             float *pp = A.part + (((x * A.c.G + g) * A.splits + split) * 16 + rr) * (D + 4);
-            *reinterpret_cast<float4 *>(pp + d) = make_float4(o[0], o[1], o[2], o[3]);
-            if (d == 0) *reinterpret_cast<float2 *>(pp + D) = make_float2(M, L);
+            if (A.tickets != nullptr) {
+                put2(pp + d, o[0], o[1]);
+                put2(pp + d + 2, o[2], o[3]);
+                if (d == 0) put2(pp + D, M, L);
+            } else {
+                *reinterpret_cast<float4 *>(pp + d) = make_float4(o[0], o[1], o[2], o[3]);
+                if (d == 0) *reinterpret_cast<float2 *>(pp + D) = make_float2(M, L);
+            }
             continue;
         }
         store_out4<BF16>(A.out, out_at(A, rt, g, rr, D) + d, o, inverse(L));
     }
+    if (R.used == 1 || A.tickets == nullptr) return;
+    // the workgroup that finishes a row tile and head last joins its splits and leaves the ticket at zero
+    __shared__ int last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                    // this thread's partials have arrived
+    __syncthreads();
+    int32_t *ticket = A.tickets + x * A.c.G + g;
+    if (tid == 0) last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == R.used - 1;
+    __syncthreads();
+    if (!last) return;
+    if (tid == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    join_rows<16, D, BF16, true>(A, rt, x, g, R.used, tid / 16);
 }
 
 // One workgroup: a tile of 128 rows (64 of fp32), 32 (16) to a wave, a kv head and a range of its key tiles.  For many
@@ -651,7 +744,8 @@ __global__ __launch_bounds__(kThreads, 2) void block_kernel(const AttnArgs A) {
     }
 #pragma unroll
     for (int c = 0; c < QT; ++c) {
-        load_query<D, BF16>(A, rt, g, w0 + c * 16 + col, T.last, q[c]);
+        load_query<D, BF16>(A, rt, g, w0 + c * 16 + col, q[c]);
+        see(A, rt, w0 + c * 16 + col, T.last, q[c]);
         shift[c] = 0.0f;
         if constexpr (OFFSET) {
             float sum = 0.0f;
@@ -752,63 +846,24 @@ __global__ __launch_bounds__(kThreads, 2) void block_kernel(const AttnArgs A) {
     }
 }
 
-// The splits of 16 rows of a row tile and head joined in order: 16 threads a row.
+// The splits of 16 rows of a row tile and head joined in order, a launch of its own.
 template <int RT, int D, bool BF16>
 __global__ __launch_bounds__(kThreads) void merge_kernel(const AttnArgs A) {
-    constexpr int V = D / 64;                        // float4 of a thread
     const int64_t x = blockIdx.x / (unsigned)A.c.G;
     const int g = (int)(blockIdx.x % (unsigned)A.c.G);
     const RowTile rt = row_tile<RT>(A, x);
     if (rt.b < 0) return;
     const int p0 = rt.len - rt.n;
     const Tiles T = visible_tiles(A, p0 + rt.r0 / A.R, p0 + (rt.r0 + rt.rows - 1) / A.R);
-    const int used = range_of(A, T.count, 0).used, rr = blockIdx.y * 16 + threadIdx.x / 16, d = (threadIdx.x & 15) * 4;
-    if (used <= 1 || rr >= rt.rows) return;
-    const int64_t step = (int64_t)RT * (D + 4);
-    const float *pp = A.part + (x * A.c.G + g) * A.splits * step + (int64_t)rr * (D + 4);
-    float M = kNeg, L = 0.0f, o[V][4] = {};
-    for (int s0 = 0; s0 < used; s0 += 8) {
-        float2 ml[8];
-        float4 v[8][V];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const float *w = pp + min(s0 + u, used - 1) * step;
-            ml[u] = *reinterpret_cast<const float2 *>(w + D);
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[u][j] = *reinterpret_cast<const float4 *>(w + j * 64 + d);
-        }
-        float now = M;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) now = fmaxf(now, ml[u].x);
-        const float f0 = __builtin_amdgcn_exp2f(M - now);
-        M = now;
-        L *= f0;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[j][i] *= f0;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const float f = s0 + u < used ? __builtin_amdgcn_exp2f(ml[u].x - M) : 0.0f;
-            L = fmaf(f, ml[u].y, L);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                o[j][0] = fmaf(f, v[u][j].x, o[j][0]);
-                o[j][1] = fmaf(f, v[u][j].y, o[j][1]);
-                o[j][2] = fmaf(f, v[u][j].z, o[j][2]);
-                o[j][3] = fmaf(f, v[u][j].w, o[j][3]);
-            }
-        }
-    }
-    const int64_t at = out_at(A, rt, g, rr, D) + d;
-#pragma unroll
-    for (int j = 0; j < V; ++j) store_out4<BF16>(A.out, at + j * 64, o[j], inverse(L));
+    const int used = range_of(A, T.count, 0).used;
+    if (used > 1) join_rows<RT, D, BF16, false>(A, rt, x, g, used, blockIdx.y * 16 + threadIdx.x / 16);
 }
 
-// How a call is split: row tiles of 16 or 128 rows, and each one's keys into ranges, so that the workgroups fill the GPU.
+// How a call is split: row tiles of 16 or 128 (64 of fp32) rows, and each one's keys into ranges of `per` tiles, so that the
+// workgroups fill the GPU.
 struct Plan {
     int64_t tiles, splits, bytes;
-    int rows;
+    int rows, per;
 };
 constexpr int64_t kMaxTokens = 1 << 30;      // positions, rows and windows fit 32 bits with room for their differences
 constexpr int kMaxSplits = 64;
@@ -816,13 +871,15 @@ Plan plan_of(int64_t N, int64_t B, int64_t H, int64_t G, bool bf16, int64_t max_
              int64_t window, int64_t n_sink) {
     Plan p;
     const int64_t R = H / G;
-    p.rows = max_new * R <= 16 ? 16 : bf16 ? kBlockRows<true> : kBlockRows<false>;
+    max_new = std::min(max_new, N);
+    p.rows = max_new * R <= 32 ? 16 : bf16 ? kBlockRows<true> : kBlockRows<false>;
     p.tiles = N * R / p.rows + B;            // a sequence's n rows make at most n R / rows + 1 tiles
     int64_t keys = max_keys;
-    if (window > 0) keys = std::min(keys, window + n_sink + max_new + 2 * kTile);
-    const int64_t most = std::max<int64_t>(1, (keys / kTile + 1) / kWaves), target = p.rows == 16 ? 1024 : 512;
-    const int64_t groups = p.tiles * G, want = p.rows == 16 ? (target + groups - 1) / groups : target / groups;
-    p.splits = std::max<int64_t>(1, std::min({want, most, (int64_t)kMaxSplits}));
+    if (window > 0 && window < kMaxTokens) keys = std::min(keys, window + std::min(n_sink, kMaxTokens) + max_new + 2 * kTile);
+    const int64_t most = std::max<int64_t>(1, (keys + kTile - 1) / kTile), groups = p.tiles * G;
+    const int64_t want = p.rows == 16 ? (1024 + groups - 1) / groups : std::max<int64_t>(1, 512 / groups);
+    p.per = (int)std::max<int64_t>(kWaves, (most + std::min<int64_t>(want, kMaxSplits) - 1) / std::min<int64_t>(want, kMaxSplits));
+    p.splits = (most + p.per - 1) / p.per;
     p.bytes = p.splits > 1 ? p.tiles * G * p.splits * p.rows * (D + 4) * 4 : 0;
     return p;
 }
@@ -845,6 +902,15 @@ int vgx_paged_attn(const vgx_paged_kv *kv, int64_t layer, int dtype, const void 
                    int64_t N, int64_t H, const int32_t *table, int64_t ldt, int64_t table_cols, const int32_t *lens,
                    const int32_t *q_start, int64_t B, int64_t max_new, int64_t max_keys, int64_t window, int64_t n_sink,
                    float scale, void *workspace, int64_t workspace_bytes, void *stream) {
+    return vgx_paged_attn_tickets(kv, layer, dtype, q, ldq, out, ldo, N, H, table, ldt, table_cols, lens, q_start, B, max_new,
+                                  max_keys, window, n_sink, scale, workspace, workspace_bytes, nullptr, 0, stream);
+}
+
+int vgx_paged_attn_tickets(const vgx_paged_kv *kv, int64_t layer, int dtype, const void *q, int64_t ldq, void *out,
+                           int64_t ldo, int64_t N, int64_t H, const int32_t *table, int64_t ldt, int64_t table_cols,
+                           const int32_t *lens, const int32_t *q_start, int64_t B, int64_t max_new, int64_t max_keys,
+                           int64_t window, int64_t n_sink, float scale, void *workspace, int64_t workspace_bytes,
+                           int32_t *tickets, int64_t n_tickets, void *stream) {
     if (const int rc = check_paged(kv, layer)) return rc;
     if (dtype != VGX_F32 && dtype != VGX_BF16) return VGX_E_DTYPE;
     if (!q_start && N != B) return VGX_E_SIZE;
@@ -860,11 +926,14 @@ int vgx_paged_attn(const vgx_paged_kv *kv, int64_t layer, int dtype, const void 
     if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return VGX_E_ARENA;
     const Plan p = plan_of(N, B, H, kv->G, dtype == VGX_BF16, max_new, max_keys, kv->D, window, n_sink);
     if (p.tiles * kv->G > 0x7FFFFFFF) return VGX_E_LIMIT;
+    if (n_tickets < 0) return VGX_E_SIZE;
+    if ((uintptr_t)tickets % 4) return VGX_E_ALIGN;
+    // few rows a tile: a launch saved; more, and their states are too many for the one workgroup that would join them
+    int32_t *mine = p.rows == 16 && n_tickets >= p.tiles * kv->G ? tickets : nullptr;
     // no position reaches kMaxTokens: a window of that many tokens is none
     const int win = window >= kMaxTokens ? 0 : (int)window, sink = (int)std::min(n_sink, kMaxTokens);
     const AttnArgs A{paged_layer(kv, layer), q, out, ldq, ldo, ldt, table, lens, q_start, static_cast<float *>(workspace),
-                     scale, (int)N, (int)B, (int)H, (int)(H / kv->G), (int)table_cols, win, sink,
-                     (int)p.splits, kWaves};
+                     scale, mine, (int)N, (int)B, (int)H, (int)(H / kv->G), (int)table_cols, win, sink, (int)p.splits, p.per};
     const int64_t tiles = q_start ? p.tiles : B * ((H / kv->G + p.rows - 1) / p.rows);
     const dim3 grid((unsigned)(tiles * kv->G), (unsigned)p.splits);
     const auto launch = [&](auto fm, auto dm, auto bf) -> int {
@@ -873,7 +942,7 @@ int vgx_paged_attn(const vgx_paged_kv *kv, int64_t layer, int dtype, const void 
         if (p.rows == 16) one ? run(rows_kernel<fm.value, dm.value, bf.value, true>) : run(rows_kernel<fm.value, dm.value, bf.value, false>);
         else one ? run(block_kernel<fm.value, dm.value, bf.value, true>) : run(block_kernel<fm.value, dm.value, bf.value, false>);
         VGX_CHECK_LAUNCH();
-        if (p.splits == 1) return VGX_OK;
+        if (p.splits == 1 || mine) return VGX_OK;
         if (p.rows == 16)
             hipLaunchKernelGGL((merge_kernel<16, dm.value, bf.value>), dim3(grid.x, 1), dim3(kThreads), 0,
                                (hipStream_t)stream, A);

@@ -299,18 +299,28 @@ def embed(w: QWeight, ids: torch.Tensor, pad_row: int = 0, out: Optional[torch.T
 KV_DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 
 
+TICKETS = 16384
+
+
 class Workspace:
     """Grow-only device scratch owned by the caller (the library never allocates)."""
 
     def __init__(self, device):
         self.device = device
         self.buf = torch.empty(0, dtype=torch.uint8, device=device)
+        self.marks = None
 
     def get(self, nbytes: int) -> torch.Tensor:
         """At least ``nbytes`` bytes (256-byte aligned, zero-filled when first allocated)."""
         if self.buf.numel() < nbytes:
             self.buf = torch.zeros(max(nbytes, 2 * self.buf.numel()), dtype=torch.uint8, device=self.device)
         return self.buf
+
+    def tickets(self) -> torch.Tensor:
+        """int32 zeros for kernels that count finished workgroups and leave them at zero, apart from the scratch."""
+        if self.marks is None:
+            self.marks = torch.zeros(TICKETS, dtype=torch.int32, device=self.device)
+        return self.marks
 
 
 def attn_decode(q: torch.Tensor, spans, out: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,

@@ -20,7 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from .ops import KV_DTYPES, Workspace, _on, _ptr, _stream
+from .ops import KV_DTYPES, TICKETS, Workspace, _on, _ptr, _stream
 
 I8, E4M3 = L.I8, L.E4M3
 PAGES = (16, 32, 64, 128, 256)
@@ -248,12 +248,14 @@ def attend(kv: PagedKV, layer: int, q: torch.Tensor, table: torch.Tensor, lens: 
         if buf.get_device() != kv.index:
             raise ValueError("the workspace must be on the cache's device")
         need = buf.numel()
+    marks, n_marks = (ws.tickets().data_ptr(), TICKETS) if buf is not None and ws is not None else (None, 0)
     with _on(kv.device):
-        rc = kv.lib.vgx_paged_attn(kv.ref, layer, dt, src.data_ptr(), _ld(src), out.data_ptr(), _ld(out), N, H,
-                                   table.data_ptr(), ldt, cols, lens.data_ptr(), _ptr(q_start), B, most, keys, window, n_sink,
-                                   D ** -0.5 if scale is None else scale, _ptr(buf), need, _stream(kv.device))
+        rc = kv.lib.vgx_paged_attn_tickets(kv.ref, layer, dt, src.data_ptr(), _ld(src), out.data_ptr(), _ld(out), N, H,
+                                           table.data_ptr(), ldt, cols, lens.data_ptr(), _ptr(q_start), B, most, keys, window,
+                                           n_sink, D ** -0.5 if scale is None else scale, _ptr(buf), need, marks, n_marks,
+                                           _stream(kv.device))
     if rc:
-        L.check(rc, "vgx_paged_attn")
+        L.check(rc, "vgx_paged_attn_tickets")
     return out
 
 
