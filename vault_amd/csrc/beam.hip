@@ -105,10 +105,11 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(const float *__restrict
     __syncthreads();
     if (lane == 0) red[wave] = s;
 
-    // the K-th largest of the lanes' maxima, bit by bit
+    // the K-th largest of the lanes' maxima, bit by bit; 15 bits of the mantissa will do (a value more may reach the bound)
     const uint32_t mine = ordered(top);
     uint32_t bound = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+#pragma unroll
+    for (int bit = 31; bit >= 8; --bit) {
         const uint32_t t = bound | (1u << bit);
         if (__popcll(__ballot(mine >= t)) >= K) bound = t;
     }

@@ -103,36 +103,43 @@ def _table(t: torch.Tensor, kv: PagedKV, name: str = "table") -> Tuple[int, int,
     return B, n, ld
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    """Whether [N, heads, D] has contiguous heads and 16-byte aligned rows."""
+def _stride(t: torch.Tensor, N: int, H: int, D: int) -> int:
+    """The row stride of t [N, H, D] if its heads are contiguous and its rows 16-byte aligned, else 0."""
     if t.data_ptr() % 16:
-        return False
+        return 0
     if t.is_contiguous():
-        return True
-    N, H, D = t.shape
+        return H * D
     st = t.stride()
-    return st[2] == 1 and (H == 1 or st[1] == D) and (N == 1 or (st[0] * t.element_size() % 16 == 0 and st[0] >= H * D))
+    if st[2] != 1 or (H > 1 and st[1] != D):
+        return 0
+    if N == 1:
+        return H * D
+    return st[0] if st[0] * t.element_size() % 16 == 0 and st[0] >= H * D else 0
 
 
-def _rows(t: torch.Tensor, heads: Optional[int], dtype, kv: PagedKV, name: str) -> torch.Tensor:
-    """[N, heads, D] with contiguous heads and 16-byte aligned rows (a copy where the view is not)."""
-    if t.dim() != 3 or t.shape[2] != kv.D or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [N, {heads if heads is not None else 'H'}, {kv.D}], got {tuple(t.shape)}")
+def _rows(t: torch.Tensor, heads: int, dtype, kv: PagedKV, name: str) -> Tuple[torch.Tensor, int, int, int]:
+    """t [N, heads, D] (any number of heads where ``heads`` is 0) with contiguous heads and 16-byte aligned rows, a copy
+    where the view is not; its row stride, N and heads."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != kv.D or shape[1] < 1 or (heads and shape[1] != heads):
+        raise ValueError(f"{name} must be [N, {heads or 'H'}, {kv.D}], got {tuple(shape)}")
     if t.dtype is not dtype or t.get_device() != kv.index:
         raise ValueError(f"{name} must be {dtype} on the cache's device")
-    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
+    N, H, D = shape
+    ld = _stride(t, N, H, D)
+    if not ld:
+        t, ld = t.clone(memory_format=torch.contiguous_format), H * D
+    return t, ld, N, H
 
 
-def _dest(t: torch.Tensor, like: torch.Tensor, name: str) -> None:
-    """An output that rows are written into, in place."""
-    if t.shape != like.shape or t.dtype is not like.dtype or t.get_device() != like.get_device():
-        raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on the cache's device")
-    if not _aligned(t):
+def _dest(t: torch.Tensor, N: int, H: int, dtype, kv: PagedKV, name: str) -> int:
+    """The row stride of an output that rows are written into, in place."""
+    if t.shape != (N, H, kv.D) or t.dtype is not dtype or t.get_device() != kv.index:
+        raise ValueError(f"{name} must be {(N, H, kv.D)} {dtype} on the cache's device")
+    ld = _stride(t, N, H, kv.D)
+    if not ld:
         raise ValueError(f"{name} needs contiguous heads and 16-byte aligned rows")
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return ld
 
 
 def _batch(q_start: Optional[torch.Tensor], B: int, N: int, kv: PagedKV) -> None:
@@ -171,9 +178,10 @@ def append(kv: PagedKV, layer: int, k: torch.Tensor, v: torch.Tensor, table: tor
     dt = KV_DTYPES.get(k.dtype)
     if dt is None:
         raise ValueError("k must be fp32 or bf16")
-    k, v = _rows(k, kv.G, k.dtype, kv, "k"), _rows(v, kv.G, k.dtype, kv, "v")
-    N = k.shape[0]
-    if v.shape[0] != N:
+    dtype = k.dtype
+    k, ldk, N, _ = _rows(k, kv.G, dtype, kv, "k")
+    v, ldv, n, _ = _rows(v, kv.G, dtype, kv, "v")
+    if n != N:
         raise ValueError("k and v must have the same rows")
     _batch(q_start, B, N, kv)
     _words(start, B, kv, "start")
@@ -186,19 +194,17 @@ def append(kv: PagedKV, layer: int, k: torch.Tensor, v: torch.Tensor, table: tor
             raise ValueError("rope rows must be contiguous, apart and 16-byte aligned")
     src = None
     if q is not None:
-        src = _rows(q, None, k.dtype, kv, "q")
-        if src.shape[0] != N or src.shape[1] < 1:
+        src, ldq, n, H = _rows(q, 0, dtype, kv, "q")
+        if n != N:
             raise ValueError("q must have the rows of k")
-        H = src.shape[1]
         if q_out is None:
-            q_out = torch.empty(N, H, D, dtype=k.dtype, device=kv.device)
+            q_out, ldqo = torch.empty(N, H, D, dtype=dtype, device=kv.device), H * D
         else:
-            _dest(q_out, q, "q_out")
-        ldq, ldqo = _ld(src), _ld(q_out)
+            ldqo = _dest(q_out, N, H, dtype, kv, "q_out")
     elif q_out is not None:
         raise ValueError("q_out without q")
     with _on(kv.device):
-        rc = kv.lib.vgx_paged_append(kv.ref, layer, dt, k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), N, table.data_ptr(), ldt,
+        rc = kv.lib.vgx_paged_append(kv.ref, layer, dt, k.data_ptr(), ldk, v.data_ptr(), ldv, N, table.data_ptr(), ldt,
                                      cols, start.data_ptr(), _ptr(q_start), B, _ptr(rope), rope_ld, rope_rows, _ptr(src), ldq,
                                      _ptr(q_out), ldqo, H, _stream(kv.device))
     if rc:
@@ -224,18 +230,18 @@ def attend(kv: PagedKV, layer: int, q: torch.Tensor, table: torch.Tensor, lens: 
     dt = KV_DTYPES.get(q.dtype)
     if dt is None:
         raise ValueError("q must be fp32 or bf16")
-    src = _rows(q, None, q.dtype, kv, "q")
-    N, H = src.shape[0], src.shape[1]
-    if H < 1 or H % kv.G:
+    dtype = q.dtype
+    q, ldq, N, H = _rows(q, 0, dtype, kv, "q")
+    if H % kv.G:
         raise ValueError(f"{H} query heads for {kv.G} kv heads")
     _batch(q_start, B, N, kv)
     _words(lens, B, kv, "lens")
     if window < 0 or n_sink < 0:
         raise ValueError("window and n_sink must not be negative")
     if out is None:
-        out = torch.empty(N, H, D, dtype=q.dtype, device=kv.device)
+        out, ldo = torch.empty(N, H, D, dtype=dtype, device=kv.device), H * D
     else:
-        _dest(out, q, "out")
+        ldo = _dest(out, N, H, dtype, kv, "out")
     most = 1 if q_start is None else N if max_new is None else max_new
     keys = cols * kv.page
     keys = keys if max_keys is None else min(max_keys, keys)
@@ -250,7 +256,7 @@ def attend(kv: PagedKV, layer: int, q: torch.Tensor, table: torch.Tensor, lens: 
         need = buf.numel()
     marks, n_marks = (ws.tickets().data_ptr(), TICKETS) if buf is not None and ws is not None else (None, 0)
     with _on(kv.device):
-        rc = kv.lib.vgx_paged_attn_tickets(kv.ref, layer, dt, src.data_ptr(), _ld(src), out.data_ptr(), _ld(out), N, H,
+        rc = kv.lib.vgx_paged_attn_tickets(kv.ref, layer, dt, q.data_ptr(), ldq, out.data_ptr(), ldo, N, H,
                                            table.data_ptr(), ldt, cols, lens.data_ptr(), _ptr(q_start), B, most, keys, window,
                                            n_sink, D ** -0.5 if scale is None else scale, _ptr(buf), need, marks, n_marks,
                                            _stream(kv.device))
