@@ -332,12 +332,12 @@ typedef struct vgx_paged_kv {
  * [B + 1], not decreasing; NULL: N == B, one row each), at the positions start[b] (device int32), start[b] + 1, ...
  * Rows from q_start[B] on, and tokens at a position below 0 or without a page, are skipped.
  * With `rope` (fp32 rows [cos(D/2) | sin(D/2)], row stride rope_ld; row p for position p) keys are rotated on the way
- * (fp32 products and sums rounded once); a position outside [0, rope_rows) counts as NaN.
+ * (products and their sum rounded once, to fp32); a position outside [0, rope_rows) counts as NaN.
  * A page's scale becomes max(its scale, if it holds tokens before start[b]; amax / 127 or amax / 448 over its new
  * tokens), amax the largest magnitude of head g; new codes are round(fp32(x / scale)), to nearest even, and the codes of
  * the older tokens are rounded again when the scale grew.  A non-finite value makes the scale of its page and head NaN.
- * q (may be NULL; [H][D] per row, row stride ldq) is rotated into q_out (row stride ldqo; may be q itself).  Rows must
- * be 16-byte aligned. */
+ * q (may be NULL; [H][D] per row, row stride ldq) is rotated into q_out (row stride ldqo; may be q itself) in fp32
+ * arithmetic, at every position from 0 on, with a page or without.  Rows must be 16-byte aligned. */
 int vgx_paged_append(const vgx_paged_kv *kv, int64_t layer, int dtype, const void *k, int64_t ldk, const void *v,
                      int64_t ldv, int64_t N, const int32_t *table, int64_t ldt, int64_t table_cols, const int32_t *start,
                      const int32_t *q_start, int64_t B, const float *rope, int64_t rope_ld, int64_t rope_rows,
@@ -348,11 +348,11 @@ int vgx_paged_append(const vgx_paged_kv *kv, int64_t layer, int dtype, const voi
  *   out[row, h] = softmax_j(scale * q[row, h] . k_j) v_j    over keys j <= p of head h / (H / G) with a page and, when
  * window > 0, with j > p - window or j < n_sink (the first tokens that stay visible).  A row that sees no key gets
  * zeros; rows from q_start[B] on are left as they are.  q and out: dtype VGX_F32 (fp32-level results) or VGX_BF16 (fp32
- * sums, probabilities in fp16); head h of a row at h * D.  Rows must be 16-byte aligned, H a multiple of G.
+ * sums, probabilities in fp16); head h of a row at h * D; out may be q.  Rows must be 16-byte aligned, H a multiple of G.
  * max_new: the most rows of a sequence, max_keys: the most keys of one (hints that choose how the work is split;
  * results do not depend on their truth beyond rounding).  workspace: vgx_paged_attn_workspace_bytes of the same
- * arguments, 16-byte aligned, any content; calls sharing one must not overlap in time.  N, B, max_keys <= 2^30 and
- * table_cols * page < 2^30. */
+ * arguments, 16-byte aligned, any content; calls sharing one must not overlap in time.  N * H / G, B, max_keys <= 2^30
+ * and table_cols * page < 2^30. */
 int64_t vgx_paged_attn_workspace_bytes(int64_t N, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_new,
                                        int64_t max_keys, int64_t window, int64_t n_sink);
 int vgx_paged_attn(const vgx_paged_kv *kv, int64_t layer, int dtype, const void *q, int64_t ldq, void *out, int64_t ldo,
@@ -594,8 +594,9 @@ int vgx_sample_topk(const float *logits, int64_t ld, int64_t B, int64_t V, int64
                     int64_t *out, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Beam search's choice: for groups of K beams (K <= 64; logits row b * K + k, row stride ld) the K best of the K * V
- * continuations by total(k, v) = scores[b * K + k] + x_v - log(sum_u exp(x_u)), in descending order, ties to the smaller
- * k * V + v.  A beam with done[b * K + k] != 0 (done may be NULL) has the one continuation (k, eos) with total =
+ * continuations by total(k, v) = scores[b * K + k] + x_v - log(sum_u exp(x_u)) in fp64 (the sum of a few thousand
+ * exponentials each in fp32), in descending order, ties to the smaller k * V + v (of one beam's continuations, to the
+ * larger x first, whose totals may be equal after rounding).  A beam with done[b * K + k] != 0 (done may be NULL) has the one continuation (k, eos) with total =
  * its score.  Totals that are NaN or -inf are no candidates.  Writes scores_out (fp32), parents (the beam k), tokens
  * (int64) and, unless NULL, done_out (the parent's flag, or token == eos); where candidates run out: -inf, the beam's
  * own index, token -1, done 1.  eos < 0: none (done must then be NULL).  V <= 2^19.  scores_out and done_out may be

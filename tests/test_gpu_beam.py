@@ -27,7 +27,7 @@ def _check(dev, x, s, done=None, eos=-1, ws=None):
 
 
 @pytest.mark.parametrize("B,K,V", [(1, 1, 1), (1, 4, 5), (3, 4, 1000), (2, 8, 4096), (2, 8, 4097), (5, 3, 8191), (1, 64, 3000),
-                                   (2, 33, 20000), (1, 5, 151665), (16, 8, 70001), (1, 64, 64), (1, 2, 1 << 19)])
+                                   (2, 33, 20000), (1, 5, 151665), (16, 8, 70001), (1, 64, 64), (1, 2, 1 << 19), (1, 33, 1 << 19)])
 def test_select(dev, B, K, V):
     rng = np.random.default_rng(B * K + V)
     x = (rng.standard_normal((B * K, V)) * 3).astype(np.float32)

@@ -684,3 +684,57 @@ def test_captured_splits(dev):
         got = out.clone()
         assert torch.equal(got, paged.attend(kv, 1, q, t, lens, ws=ws)) and torch.equal(got, paged.attend(kv, 1, q, t, lens))
         assert not ws.tickets().any() and (n > 0 or not got.any())
+
+
+def test_workspace_first_used_in_a_capture(dev):
+    """A workspace whose first user is a capture, then an eager call before any replay, then replays."""
+    rng = np.random.default_rng(33)
+    D, P, G, H = 64, 32, 2, 8
+    c = _garbage(rng, 100, G, P, D, "i8")
+    table = _table(rng, [3000], P, 100)
+    _fill(rng, c, table, [3000])
+    kv, t, lens = _to(c, dev), _i32(table, dev), _i32([3000], dev)
+    q, ws = torch.randn(1, H, D, device=dev), ops.Workspace(dev)
+    want = paged.attend(kv, 1, q, t, lens)
+    graph = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=s):
+        out = paged.attend(kv, 1, q, t, lens, ws=ws)
+    assert torch.equal(paged.attend(kv, 1, q, t, lens, ws=ws), want)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(paged.attend(kv, 1, q, t, lens, ws=ws), want) and not ws.tickets().any()
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("lens,counts", [([2600], [1]), ([700, 5, 90], [9, 1, 30]), ([40], [40])])
+def test_attend_in_place(dev, lens, counts, dt):
+    """out is q: the same bits as into another tensor, split or not, with few rows and many."""
+    rng = np.random.default_rng(34)
+    D, P, G, H, N = 128, 32, 2, 12, sum(counts)
+    c = _garbage(rng, 110, G, P, D, "e4m3")
+    table = _table(rng, lens, P, 110)
+    _fill(rng, c, table, lens)
+    kv, t, n, ws = _to(c, dev), _i32(table, dev), _i32(lens, dev), ops.Workspace(dev)
+    q = torch.from_numpy(rng.standard_normal((N, H, D)).astype(np.float32)).to(DT[dt]).to(dev)
+    for most in (2, max(counts)):
+        for w in (None, ws):
+            kw = dict(q_start=_starts(counts, dev), max_new=most, ws=w)
+            want, y = paged.attend(kv, 1, q, t, n, **kw), q.clone()
+            assert paged.attend(kv, 1, y, t, n, out=y, **kw) is y and torch.equal(y, want)
+
+
+def test_attend_lowest_lengths(dev):
+    """Lengths below 0 down to the type's lowest: nothing is visible."""
+    kv = paged.PagedKV.empty(1, 4, 1, 64, dev, page=16)
+    for t in (kv.k, kv.v, kv.k_scale, kv.v_scale):
+        t.fill_(7)
+    table = _i32([[0, 1, 2, 3]] * 3, dev)
+    for low in (-1, -(1 << 31) + 1, -(1 << 31)):
+        for counts in ([1, 1, 1], [2, 0, 90]):
+            got = paged.attend(kv, 0, torch.randn(sum(counts), 2, 64, device=dev), table, _i32([low] * 3, dev),
+                               q_start=_starts(counts, dev))
+            assert not got.any()

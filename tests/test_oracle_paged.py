@@ -207,3 +207,20 @@ def test_refused_tickets():
     for kw, code in [(dict(n=-1), -1), (dict(tickets=p + 2), -11), (dict(out=None), -31), (dict(H=13), -7), (dict(ldq=1), -1)]:
         assert lib.vgx_paged_attn_tickets(C.byref(kv), *dict(base, **kw).values(), None) == code, kw
     assert lib.vgx_paged_attn_tickets(C.byref(kv), *dict(base, N=0).values(), None) == 0
+
+
+def test_refused_sizes():
+    """Launches of 2^32 threads and more, and rows whose number does not fit 32 bits."""
+    lib, kv = L.load(), C.byref(_kv())
+    n, wide = 1 << 29, 1 << 20
+    bytes_of = lib.vgx_paged_attn_workspace_bytes
+    assert bytes_of(n, 1, 8, 2, 64, n, 64, 0, 0) == -10 and bytes_of(n, 1, 4, 2, 64, n, 64, 0, 0) >= 0
+    assert lib.vgx_paged_attn(kv, 0, L.BF16, p, 1536, p, 1536, 1 << 24, 12, p, 4, 4, p, None, 1 << 24, 1, 64, 0, 0, 1.0, p,
+                              1 << 62, None) == -10
+    assert lib.vgx_paged_append(kv, 0, L.F32, p, 256, p, 256, 1 << 24, p, 4, 4, p, None, 1 << 24, None, 0, 0, None, 0, None,
+                                0, 0, None) == -10
+    assert lib.vgx_paged_read(kv, L.F32, p, 4, 4, p, p, 1 << 62, 5, p, p, None) == -10
+    small = C.byref(_kv(page=16))
+    assert lib.vgx_paged_read(small, L.F32, p, 4, 4, p, p, 1, 1 << 28, p, p, None) == -10
+    for groups in (wide, 1 << 24, 1 << 62):
+        assert lib.vgx_paged_reorder(kv, p, 4, 4, p, p, groups, 64, p + 64, 4, p + 64, None) == -10

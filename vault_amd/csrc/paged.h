@@ -9,6 +9,7 @@
 
 namespace vgx {
 
+constexpr int64_t kMaxGroups = (1 << 24) - 1;      // workgroups of 256 threads in a launch of less than 2^32 threads
 constexpr float kQMaxI8 = 127.0f, kQMaxE4M3 = 448.0f;
 
 // A layer's pages as kernels see them.

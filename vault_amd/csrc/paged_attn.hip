@@ -73,7 +73,7 @@ VGX_DEV RowTile row_tile(const AttnArgs &A, int64_t x) {
     t.n = r.hi - r.lo;
     t.r0 = __builtin_amdgcn_readfirstlane((int)place) * RT;
     t.rows = (int)min((int64_t)RT, (int64_t)t.n * A.R - t.r0);
-    t.len = A.lens[t.b];
+    t.len = max(A.lens[t.b], 0);            // so that positions, which are len - n and on, fit 32 bits
     return t;
 }
 
@@ -908,7 +908,7 @@ int64_t vgx_paged_attn_workspace_bytes(int64_t N, int64_t B, int64_t H, int64_t 
                                        int64_t max_keys, int64_t window, int64_t n_sink) {
     if (N < 0 || B < 0 || H <= 0 || G <= 0 || max_new < 0 || max_keys < 0 || window < 0 || n_sink < 0) return VGX_E_SIZE;
     if (H % G || (D != 64 && D != 128)) return VGX_E_SHAPE;
-    if (N > kMaxTokens || B > kMaxTokens || H > 65535 || max_keys > kMaxTokens) return VGX_E_LIMIT;
+    if (N > kMaxTokens || B > kMaxTokens || H > 65535 || max_keys > kMaxTokens || N * (H / G) > kMaxTokens) return VGX_E_LIMIT;
     if (N == 0 || B == 0) return 0;
     return std::max(plan_of(N, B, H, G, false, max_new, max_keys, D, window, n_sink).bytes,
                     plan_of(N, B, H, G, true, max_new, max_keys, D, window, n_sink).bytes);
@@ -941,7 +941,7 @@ int vgx_paged_attn_tickets(const vgx_paged_kv *kv, int64_t layer, int dtype, con
     if (((uintptr_t)q | (uintptr_t)out) % 16 || ldq * es % 16 || ldo * es % 16) return VGX_E_ALIGN;
     if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return VGX_E_ARENA;
     const Plan p = plan_of(N, B, H, kv->G, dtype == VGX_BF16, max_new, max_keys, kv->D, window, n_sink);
-    if (p.tiles * kv->G > 0x7FFFFFFF) return VGX_E_LIMIT;
+    if (p.tiles * kv->G > kMaxGroups) return VGX_E_LIMIT;
     if (n_tickets < 0) return VGX_E_SIZE;
     if ((uintptr_t)tickets % 4) return VGX_E_ALIGN;
     // few rows a tile: a launch saved; more, and their states are too many for the one workgroup that would join them

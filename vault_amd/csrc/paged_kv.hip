@@ -54,7 +54,7 @@ struct PageRun {
 };
 
 // Four dims of a K row from d and four from d + D / 2, rotated: products and sum in fp64, rounded once, so that the
-// codes are those of the definition and not of an order of fp32 operations.
+// codes are those of the definition and not of an order of fp32 operations.  (Queries are not rounded to codes: fp32.)
 template <bool BF16, int D>
 VGX_DEV void rotated8(const AppendArgs &A, int64_t row, int64_t pos, int g, int d, float (&lo)[4], float (&hi)[4]) {
     float a[4], b[4];
@@ -197,8 +197,8 @@ VGX_DEV void rotate_query(const AppendArgs &A, int64_t row) {
 // then hold them between the search for the largest magnitude and the rounding; otherwise they are read again.  V's codes
 // are turned from tokens to dims in registers, four by four, and pass through shared memory (rows of page + 4 bytes, so
 // that the dims of a wave's words lie in different banks) on their way to whole 16-byte pieces.  What bounds it is the
-// rotated queries' traffic: 13057 tokens of 32 / 8 heads in bf16, 223 MB, 63 us when every thread took two loads of its
-// rotation for 8 values of q and the tokens were read twice.
+// rotated queries' traffic: 13057 tokens of 32 / 8 heads in bf16 37 us; 63 when every thread took two loads of its rotation
+// for 8 values of q and the tokens were read twice.
 template <int FMT, int D, bool BF16, bool ONCE>
 __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs A) {
     __shared__ uint32_t red[4];
@@ -490,7 +490,7 @@ int vgx_paged_append(const vgx_paged_kv *kv, int64_t layer, int dtype, const voi
     const int64_t slots = q_start ? std::min(N, N / kv->page + 2 * B) : B;
     A.kv_groups = slots * kv->G;
     const int64_t groups = A.kv_groups + (q ? (N + 3) / 4 : 0);
-    if (groups > 0x7FFFFFFF) return VGX_E_LIMIT;
+    if (groups > kMaxGroups) return VGX_E_LIMIT;
     return with_format(kv->fmt, kv->D, dtype == VGX_BF16, [&](auto fm, auto dm, auto bf) -> int {
         const auto run = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kThreads), (size_t)(kv->D * (kv->page + 4)),
@@ -514,12 +514,12 @@ int vgx_paged_read(const vgx_paged_kv *kv, int dtype, const int32_t *table, int6
     if (const int rc = check_table(table, ldt, table_cols)) return rc;
     if (!first || !lens || !k_out || !v_out) return VGX_E_ARG;
     if (((uintptr_t)k_out | (uintptr_t)v_out) % 16) return VGX_E_ALIGN;
-    if (n > 0x3FFFFFFF || B * kv->G > 65535) return VGX_E_LIMIT;
+    const int64_t pages = (std::min<int64_t>(n, 1 << 30) + kv->page - 2) / kv->page + 1;
+    if (n > 0x3FFFFFFF || pages > kMaxGroups || B > 65535 || B * kv->G > 65535) return VGX_E_LIMIT;
     const int log_page = paged_layer(kv, 0).log_page;
-    const unsigned pages = (unsigned)((n + kv->page - 2) / kv->page + 1);
     return with_format(kv->fmt, kv->D, dtype == VGX_BF16, [&](auto fm, auto dm, auto bf) -> int {
         hipLaunchKernelGGL((read_kernel<fm.value, dm.value, bf.value>),
-                           dim3(pages, (unsigned)(B * kv->G), (unsigned)kv->n_layers), dim3(kThreads),
+                           dim3((unsigned)pages, (unsigned)(B * kv->G), (unsigned)kv->n_layers), dim3(kThreads),
                            (size_t)(kv->D * (kv->page + 4)), (hipStream_t)stream, *kv, log_page, table, ldt, (int)table_cols,
                            first, lens, (int)n, k_out, v_out);
         VGX_CHECK_LAUNCH();
@@ -537,7 +537,7 @@ int vgx_paged_reorder(const vgx_paged_kv *kv, const int32_t *table, int64_t ldt,
     if (const int rc = check_table(table, ldt, table_cols)) return rc;
     if (const int rc = check_table(table_out, ldt_out, table_cols)) return rc;
     if (!lens || !parents || !lens_out || table_out == table || lens_out == lens) return VGX_E_ARG;
-    if (groups * K > 0x7FFFFFFF || kv->n_layers >= 65535) return VGX_E_LIMIT;
+    if (groups > kMaxGroups || groups * K > kMaxGroups || kv->n_layers >= 65535) return VGX_E_LIMIT;
     const int log_page = paged_layer(kv, 0).log_page;
     // 16 KB of K and of V to a workgroup
     const unsigned slices = (unsigned)std::min<int64_t>(16, std::max<int64_t>(1, kv->G * kv->page * kv->D / 16384));

@@ -316,9 +316,12 @@ class Workspace:
             self.buf = torch.zeros(max(nbytes, 2 * self.buf.numel()), dtype=torch.uint8, device=self.device)
         return self.buf
 
-    def tickets(self) -> torch.Tensor:
-        """int32 zeros for kernels that count finished workgroups and leave them at zero, apart from the scratch."""
+    def tickets(self) -> Optional[torch.Tensor]:
+        """int32 zeros for kernels that count finished workgroups and leave them at zero, apart from the scratch.  None
+        if a capture asks first: what it records sets them to zero at its replay only."""
         if self.marks is None:
+            if torch.cuda.is_current_stream_capturing():
+                return None
             self.marks = torch.zeros(TICKETS, dtype=torch.int32, device=self.device)
         return self.marks
 
@@ -831,6 +834,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: Optional[torch
     (B, K), V, dev = scores.shape, logits.shape[1], logits.device
     need = _beam_bytes(B, K, V)
     buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=dev)
+    if buf.get_device() != index:
+        raise ValueError("the workspace must be on the logits' device")
     out = torch.empty_like(scores)
     parents = torch.empty(B, K, dtype=torch.int32, device=dev)
     tokens = torch.empty(B, K, dtype=torch.int64, device=dev)

@@ -221,7 +221,7 @@ def attend(kv: PagedKV, layer: int, q: torch.Tensor, table: torch.Tensor, lens: 
     q [N, H, D] fp32 or bf16, rotated; lens int32 [B]: tokens that sequence b holds, its queries being its last ones (so
     after an append, lens = start + new tokens).  Every query sees the keys up to its own position, with ``window`` > 0
     only the last ``window`` of them and the first ``n_sink`` tokens.  Returns [N, H, D] in q's dtype; a query that sees
-    nothing gets zeros, rows behind the last sequence stay as they were.  ``max_new`` / ``max_keys``: the most rows and
+    nothing gets zeros, rows behind the last sequence stay as they were.  ``out`` may be q.  ``max_new`` / ``max_keys``: the most rows and
     keys of one sequence, hints for the split of the work (by default what the shapes allow).  ``ws``: a Workspace of this
     stream; without it scratch is allocated."""
     D = kv.D
@@ -254,12 +254,12 @@ def attend(kv: PagedKV, layer: int, q: torch.Tensor, table: torch.Tensor, lens: 
         if buf.get_device() != kv.index:
             raise ValueError("the workspace must be on the cache's device")
         need = buf.numel()
-    marks, n_marks = (ws.tickets().data_ptr(), TICKETS) if buf is not None and ws is not None else (None, 0)
+    marks = ws.tickets() if buf is not None and ws is not None else None
     with _on(kv.device):
         rc = kv.lib.vgx_paged_attn_tickets(kv.ref, layer, dt, q.data_ptr(), ldq, out.data_ptr(), ldo, N, H,
                                            table.data_ptr(), ldt, cols, lens.data_ptr(), _ptr(q_start), B, most, keys, window,
-                                           n_sink, D ** -0.5 if scale is None else scale, _ptr(buf), need, marks, n_marks,
-                                           _stream(kv.device))
+                                           n_sink, D ** -0.5 if scale is None else scale, _ptr(buf), need, _ptr(marks),
+                                           0 if marks is None else TICKETS, _stream(kv.device))
     if rc:
         L.check(rc, "vgx_paged_attn_tickets")
     return out
