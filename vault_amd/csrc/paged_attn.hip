@@ -889,10 +889,12 @@ Plan plan_of(int64_t N, int64_t B, int64_t H, int64_t G, bool bf16, int64_t max_
     p.tiles = N * R / p.rows + B;            // a sequence's n rows make at most n R / rows + 1 tiles
     int64_t keys = max_keys;
     if (window > 0 && window < kMaxTokens) keys = std::min(keys, window + std::min(n_sink, kMaxTokens) + max_new + 2 * kTile);
-    const int64_t most = std::max<int64_t>(1, (keys + kTile - 1) / kTile), groups = p.tiles * G;
+    const int64_t most = std::max<int64_t>(1, (keys + kTile - 1) / kTile);
+    // as many tiles as the hint allows, of which p.tiles is the bound without it
+    const int64_t groups = G * std::min(p.tiles, B * ((std::max<int64_t>(max_new, 1) * R + p.rows - 1) / p.rows));
     // 512 workgroups fill the GPU, two to a CU; where the sequences alone are as many, four times that for an even end
-    // (32 windowed sequences of 2 kv heads: 512 workgroups 19 us, 1024 25; 64 ragged ones of 8 kv heads and up to 16384
-    // tokens: 512 257 us, 1024 258, 2048 243)
+    // (32 windowed sequences of 2 kv heads: 384 workgroups 20.7 us, 512 20.0, 768 25.9; 64 of 8 kv heads and up to 16384
+    // tokens: 1024 249 us, 2048 235, 4096 235)
     const int64_t want = std::max<int64_t>(1, (p.rows == 16 && groups >= 512 ? 2048 : 512) / groups);
     p.per = (int)std::max<int64_t>(kWaves, (most + std::min<int64_t>(want, kMaxSplits) - 1) / std::min<int64_t>(want, kMaxSplits));
     p.splits = (most + p.per - 1) / p.per;
