@@ -329,8 +329,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs A) {
 }
 
 // One page of one (layer, sequence, head).  A thread has four tokens of four dims: K's words lie that way, V's are words
-// of four tokens and pass through shared memory (rows of page + 4 bytes: with rows of a page of 128 the dims of a wave
-// shared one bank, 335 us for 128 such pages of 28 layers, 1.2 GB).
+// of four tokens and pass through shared memory (rows of page + 4 bytes, so that the dims of a wave lie in different
+// banks).  The grid has a page more than a run of whole pages needs, and workgroups go to the dies and
+// their engines in turn: with the pages turned by a hash, those without work do not all meet on the same ones (one page of
+// 128 tokens of 128 sequences, 2 heads and 28 layers in fp32, 1.2 GB: 244 us, 368 without, 337 turned every four heads).
 template <int FMT, int D, bool BF16>
 __global__ __launch_bounds__(kThreads) void read_kernel(const vgx_paged_kv kv, int log_page, const int32_t *table,
                                                         int64_t ldt, int cols, const int32_t *first,
@@ -338,7 +340,8 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const vgx_paged_kv kv, i
     extern __shared__ uint8_t tile[];
     const int tid = threadIdx.x, P = 1 << log_page, S = P + 4, G = (int)kv.G;
     const int g = (int)(blockIdx.y % (unsigned)G), b = (int)(blockIdx.y / (unsigned)G), layer = blockIdx.z;
-    const int64_t f = first[b], len = lens[b], col = (f >> log_page) + blockIdx.x, p0 = col << log_page;
+    const unsigned turned = (blockIdx.x + (((blockIdx.y + blockIdx.z * gridDim.y) * 0x9E3779B1u) >> 16)) % gridDim.x;
+    const int64_t f = first[b], len = lens[b], col = (f >> log_page) + turned, p0 = col << log_page;
     const int lo = (int)max((int64_t)0, f - p0), hi = (int)min((int64_t)P, f + n - p0);   // the page's tokens to write
     if (hi <= lo) return;
     const int page = col >= 0 && col < cols ? table[(int64_t)b * ldt + col] : -1;
@@ -386,15 +389,16 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const vgx_paged_kv kv, i
     }
 }
 
-// Workgroup (beam, layer, slice of the page); those of one extra layer write the tables.  Every wave works out the group's heirs from the
-// parents: lane i is beam i.
+// Workgroup (beam, layer, slice of the page); those of one extra layer write the tables.  Every wave works out the group's
+// heirs from the parents: lane i is beam i.  Beams turn with the layer: the first beams of a group seldom copy, and a beam
+// of all layers would go to one die (16 groups of 8 beams, 28 layers, pages of 128 tokens: 40 us, 55 without).
 __global__ __launch_bounds__(kThreads) void reorder_kernel(const vgx_paged_kv kv, int log_page, const int32_t *table,
                                                            int64_t ldt, int cols, const int32_t *lens,
                                                            const int32_t *parents, int K, int32_t *table_out,
                                                            int64_t ldt_out, int32_t *lens_out) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int64_t base = (int64_t)(blockIdx.x / (unsigned)K) * K;
-    const int me = (int)(blockIdx.x % (unsigned)K);
+    const int me = (int)((blockIdx.x + blockIdx.y) % (unsigned)K);
     int par = lane < K ? parents[base + lane] : -1;
     if (lane < K && (par < 0 || par >= K)) par = lane;
     // heirs: the first child of each parent; dead: beams without children
