@@ -203,11 +203,11 @@ struct JoinArgs {
 };
 
 // One workgroup per group of beams.  Dynamic shared memory: `cells` totals and as many tags, at least K * chunks and K * K.
-// COUNT: up to 1024 of both are ranked by counting what comes before them (152 heads of 8 beams over 19 chunks: 5.5 us for
-// the launch); more are sorted, cells being a power of two (the same: 26 us).
+// COUNT: up to 1024 of both are ranked by counting what comes before them (152 heads of 8 beams over 19 chunks: 7.9 us for
+// the launch, 11.5 with one of 256 threads to a cell); more are sorted, cells being a power of two (the same: 26 us).
 template <int THREADS, bool COUNT>
 __global__ __launch_bounds__(THREADS) void join_kernel(const JoinArgs A, int cells) {
-    extern __shared__ uint64_t tot[];
+    extern __shared__ __align__(16) uint64_t tot[];
     uint32_t *tag = reinterpret_cast<uint32_t *>(tot + cells);
     __shared__ double lse[kMaxK];
     __shared__ float score[kMaxK];
@@ -273,39 +273,46 @@ __global__ __launch_bounds__(THREADS) void join_kernel(const JoinArgs A, int cel
         if (A.done_out != nullptr) A.done_out[base + i] = t == 0 || fin[k] || token == A.eos ? 1 : 0;
     };
     if constexpr (COUNT) {
-        // how many of the n cells come before (t, f); cells that are no candidates come after all others
-        const auto rank = [&](int n, uint64_t t, uint32_t f) {
+        // calls found(cell, its place) for the candidates among the n cells: a cell's place is how many come before it, two
+        // at a time (cells past the last are 0: no candidates, which come after all others), counted by `help` neighbouring
+        // lanes; a head's tag is its cell
+        const auto rank = [&](int n, bool tagged, auto found) {
+            int help = 1;
+            while (help < 16 && 2 * help * n <= THREADS) help <<= 1;
+            const int cell = tid / help, part = tid & (help - 1);
+            if (cell >= n) return;
+            const uint64_t t = tot[cell];
+            const uint32_t f = tagged ? tag[cell] : (uint32_t)cell;
             int r = 0;
+            if (t != 0) {
 #pragma unroll 8
-            for (int j = 0; j < n; ++j) {
-                const uint64_t a = tot[j];
-                const uint32_t g = tag[j];
-                r += (int)(a > t) | ((int)(a == t) & (int)(g < f));
+                for (int j = 2 * part; j < n; j += 2 * help) {
+                    const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(tot + j);
+                    const uint2 g = tagged ? *reinterpret_cast<const uint2 *>(tag + j) : make_uint2(j, j + 1);
+                    r += (int)(a.x > t) | ((int)(a.x == t) & (int)(g.x < f));
+                    r += (int)(a.y > t) | ((int)(a.y == t) & (int)(g.y < f));
+                }
             }
-            return r;
+            for (int off = help / 2; off > 0; off >>= 1) r += __shfl_xor(r, off, kWave);
+            if (t != 0 && part == 0) found(cell, r);
         };
         const uint64_t h = tid < K * C ? head_of(tid, head) : 0;
-        if (tid < K * C) {
-            tot[tid] = h;
-            tag[tid] = (uint32_t)tid;
-        }
+        if (tid < cells) tot[tid] = h;
         __syncthreads();
-        if (h != 0) {
-            const int r = rank(K * C, h, (uint32_t)tid);
-            if (r < K) pick[r] = tid;
-        }
+        rank(K * C, false, [&](int cell, int r) {
+            if (r < K) pick[r] = cell;
+        });
         __syncthreads();
         uint32_t f;
         const uint64_t t = entry_of(tid, f);
-        if (tid < K * K) {
+        if (tid < cells) {
             tot[tid] = t;
             tag[tid] = f;
         }
         const int some = __syncthreads_count(t != 0);
-        if (t != 0) {
-            const int r = rank(K * K, t, f);
-            if (r < K) write(r, t, f);
-        }
+        rank(K * K, true, [&](int cell, int r) {
+            if (r < K) write(r, tot[cell], tag[cell]);
+        });
         if (tid < K && tid >= some) write(tid, 0, 0);
     } else {
         const auto before = [&](int i, int j) { return tot[i] > tot[j] || (tot[i] == tot[j] && tag[i] < tag[j]); };
@@ -377,11 +384,12 @@ int vgx_beam_select(const float *logits, int64_t ld, int64_t groups, int64_t K, 
         hipLaunchKernelGGL((chunk_kernel<16>), grid, dim3(kThreads), 0, st, logits, ld, (int)V, (int)K, done, lists, sums);
     VGX_CHECK_LAUNCH();
     const JoinArgs A{lists, sums, scores, done, scores_out, parents, tokens, done_out, eos, (int)V, (int)K, (int)C};
-    const int most = (int)std::max(K * C, K * K);
+    const int most = (int)(std::max(K * C, K * K) + 1) & ~1;
     const auto join = [&](auto kernel, int threads, int cells) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(threads), (size_t)cells * 12, st, A, cells);
     };
-    if (most <= kThreads) {
+    // a wave for every beam's sum (4 beams over 8 chunks take 5.1 us in 256 threads)
+    if (most <= kThreads && K <= kWaves) {
         join(join_kernel<kThreads, true>, kThreads, most);
     } else if (most <= kJoinThreads) {
         join(join_kernel<kJoinThreads, true>, kJoinThreads, most);
