@@ -795,6 +795,9 @@ __global__ __launch_bounds__(kThreads, 2) void block_kernel(const AttnArgs A) {
         f32x4_t s[QT][4];
         f16x8_t pf[QT][2][PIECES];
         scores(s);
+        // the softmax before another wave's matrix instructions, which run on without being issued (1024 queries on 36864
+        // keys: 273 us, 279 at equal priorities, 276 with the products first)
+        __builtin_amdgcn_s_setprio(1);
         __builtin_amdgcn_sched_barrier(0);
         fetch_k(i + 1, std::integral_constant<int, 0>{});
         bool moved = false;
@@ -828,6 +831,7 @@ __global__ __launch_bounds__(kThreads, 2) void block_kernel(const AttnArgs A) {
         }
         __builtin_amdgcn_sched_barrier(0);             // the registers of s are free from here on
         fetch_k(i + 1, std::integral_constant<int, 1>{});
+        __builtin_amdgcn_s_setprio(0);
         values(buf, pf);
         drop_unseen(token_of(i + 1));
         stage(buf ^ 1);
