@@ -430,7 +430,11 @@ VGX_DEV void join_rows(const AttnArgs &A, const RowTile &rt, int64_t x, int g, i
         float2 ml[8], v[8][V];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const float *w = pp + min(s0 + u, used - 1) * step;
+            ml[u] = make_float2(kNeg, 0.0f);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[u][j] = make_float2(0.0f, 0.0f);
+            if (s0 + u >= used) continue;
+            const float *w = pp + (s0 + u) * step;
             ml[u] = get2<SHARED>(w + D);
 #pragma unroll
             for (int j = 0; j < V; ++j) v[u][j] = get2<SHARED>(w + j * 32 + d);
