@@ -308,7 +308,7 @@ int vgx_attn_prefill_ws(int kv_dtype, int q_dtype, int out_dtype, const vgx_attn
  * Page tables are device int32 [sequences][table_cols] (row stride ldt): entry j of a sequence's row is the page of its
  * tokens [j * page, (j + 1) * page).  An entry outside [0, n_pages), or past table_cols, is no page: nothing is written
  * there and its tokens are not visible, so entries of pages that a sliding window has left behind may be -1.  Pages may
- * be shared by sequences as long as only one of them writes to a page in a call.
+ * be shared by sequences as long as one entry of the table writes to a page in a call.
  * No counterpart in the reference, whose state tensors are dense and whose batches are in lockstep. */
 enum { VGX_I8 = 16, VGX_E4M3 = 17 };
 

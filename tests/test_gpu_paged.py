@@ -738,3 +738,39 @@ def test_attend_lowest_lengths(dev):
             got = paged.attend(kv, 0, torch.randn(sum(counts), 2, 64, device=dev), table, _i32([low] * 3, dev),
                                q_start=_starts(counts, dev))
             assert not got.any()
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("B", [64, 65, 515, 1100])
+def test_many_sequences(dev, B, dt):
+    """Batches past what a wave looks at at once, sequences without rows among them: append, attend and their rows."""
+    rng = np.random.default_rng(B)
+    D, P, G, H = 64, 16, 1, 3
+    counts = rng.choice([0, 1, 2, 7], B, p=[0.3, 0.3, 0.3, 0.1])
+    counts[-1] = 2
+    held = rng.integers(0, 20, B)
+    lens = held + counts
+    N, cols = int(counts.sum()), 2
+    table = rng.permutation(2 * B).reshape(B, cols)
+    t, starts = _i32(table, dev), _starts(counts, dev)
+    kv, one = (paged.PagedKV.empty(1, 2 * B, G, D, dev, page=P, fmt=FMT["i8"]) for _ in range(2))
+    for c in (kv, one):
+        for a in (c.k, c.v):
+            a.copy_(torch.from_numpy(np.random.default_rng(1).integers(1, 256, tuple(a.shape), np.uint8)))
+        c.k_scale.fill_(1e-9), c.v_scale.fill_(1e-9)
+    k, v = (torch.from_numpy(rng.standard_normal((N, G, D)).astype(np.float32)).to(DT[dt]).to(dev) for _ in range(2))
+    q = torch.from_numpy(rng.standard_normal((N, H, D)).astype(np.float32)).to(DT[dt]).to(dev)
+    paged.append(kv, 0, k, v, t, _i32(held, dev), q_start=starts)
+    got = paged.attend(kv, 0, q, t, _i32(lens, dev), q_start=starts, max_new=7)
+    at = np.concatenate([[0], np.cumsum(counts)])
+    for b in [0, 1, B // 2, B - 1] + list(np.flatnonzero(counts)[::max(1, B // 40)]):
+        lo, hi = at[b], at[b + 1]
+        if lo == hi:
+            continue
+        only = _starts([int(counts[b])], dev)
+        paged.append(one, 0, k[lo:hi], v[lo:hi], t[b:b + 1], _i32([held[b]], dev), q_start=only)
+        for p in table[b]:
+            assert torch.equal(kv.k[0, p], one.k[0, p]) and torch.equal(kv.v[0, p], one.v[0, p])
+            assert torch.equal(kv.k_scale[0, p], one.k_scale[0, p])
+        want = paged.attend(one, 0, q[lo:hi], t[b:b + 1], _i32([lens[b]], dev), q_start=only, max_new=7)
+        assert torch.equal(got[lo:hi], want), b

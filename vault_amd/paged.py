@@ -170,7 +170,7 @@ def append(kv: PagedKV, layer: int, k: torch.Tensor, v: torch.Tensor, table: tor
     k, v [N, G, D] fp32 or bf16; sequence b's rows take the positions start[b], start[b] + 1, ... (start int32 [B]: the
     tokens that it holds already).  ``rope`` fp32 [positions, D], rows [cos | sin]: keys are rotated by their position's
     row.  With q [N, H, D] (dtype of k) the queries are rotated too, into ``q_out`` (may be q; a new tensor by default),
-    which is returned.  A sequence's pages must be in its table row; a page that is written must be in one row only.
+    which is returned.  A sequence's pages must be in its table row; a page that is written must be in one entry only.
     ``max_new`` is not needed and only accepted for symmetry with ``attend``."""
     D = kv.D
     _layer(kv, layer)
