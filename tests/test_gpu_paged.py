@@ -774,3 +774,25 @@ def test_many_sequences(dev, B, dt):
             assert torch.equal(kv.k_scale[0, p], one.k_scale[0, p])
         want = paged.attend(one, 0, q[lo:hi], t[b:b + 1], _i32([lens[b]], dev), q_start=only, max_new=7)
         assert torch.equal(got[lo:hi], want), b
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [
+    # D, page, G, H, lens, counts, window, sinks: more than 96 query rows for a kv head
+    (128, 64, 1, 8, [700, 64, 300], [100, 40, 3], 0, 0),
+    (64, 16, 1, 3, [400, 33, 5, 1], [180, 20, 0, 1], 0, 0),
+    (128, 32, 2, 24, [500, 90], [90, 9], 64, 5),
+    (64, 128, 1, 20, [300, 7], [40, 7], 1, 0),
+    (128, 16, 3, 21, [120, 1000, 8], [150, 30, 8], 200, 33),
+    (128, 256, 1, 1, [1000], [500], 0, 0),
+    (64, 64, 2, 10, [2500], [130], 0, 0),
+])
+def test_attend_blocks_of_rows(dev, shape, fmt, dt):
+    D, P, G, H, lens, counts, window, sinks = shape
+    rng = np.random.default_rng(35)
+    pages = sum(-(-n // P) for n in lens) + 3
+    c = _garbage(rng, pages, G, P, D, fmt)
+    table = _table(rng, lens, P, pages)
+    _fill(rng, c, table, lens)
+    _attend(dev, c, table, lens, counts, H, dt, tail=2, window=window, n_sink=sinks)
